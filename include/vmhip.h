@@ -421,6 +421,59 @@ int vm_attention_decode_f32(const float* q, int64_t ldq, const float* k, int64_t
                             float* o, int64_t ldo, const uint8_t* key_mask, const int32_t* kv_row_index, int64_t kv_index_ld,
                             int rows, int H, int Lk, int dh, int q_per_kv, float scale, void* stream);
 
+/* ------------------------------------------------------------------ paged key-value cache (csrc/paged_cache.hip, csrc/paged_attention.hip)
+ * The cache of one decoder layer is k_pages, v_pages [P, Hkv, page_size, dh] (bf16 or fp32, contiguous, 16-byte aligned): a page holds page_size
+ * consecutive tokens of one request.  block_table int32 [N, M] (rows ld_table apart) names the pages of request i, -1 where there is none;
+ * lengths int32 [N] counts its cached tokens.  A token's slot is page * page_size + offset.
+ * What HF's generate() keeps as one growing tensor per layer (hf:generation/utils.py _sample, past_key_values; driven by
+ * ref:vilmedic/blocks/huggingface/decoder/evaluation.py:73-78) and vm_attention_fwd / vm_attention_decode_f32 reach through a row-index table.
+ *
+ * vm_paged_plan: one call admits new tokens (new_tokens[i] > 0), leaves rows alone (0) and releases rows (< 0), on the device and
+ * deterministically; integers only.  free_pages int32 [P] is a ring of free page numbers, ring int32 [2] = (head, count).
+ *   - rows are served in order; row i is REFUSED -- nothing about it changes, granted[i] = 0 -- when its tokens do not fit into the M pages of its
+ *     table row, when the packed token count up to it exceeds max_tokens, or when the free pages run out at it;
+ *   - accepted rows take ceil((len + new) / page_size) - ceil(len / page_size) pages from the head of the ring into their table row, lengths[i]
+ *     grows, granted[i] = new_tokens[i];
+ *   - released rows put their pages behind the ring's tail in (row, column) order (usable from the NEXT call on), their table row becomes -1,
+ *     lengths[i] = 0, granted[i] = 0;
+ *   - cu_tokens int32 [N + 1]: prefix sums of max(new_tokens, 0), clipped to max_tokens: the packed token order;
+ *   - slots int64 [max_tokens]: where token t of the packed order goes, -1 for refused rows and behind the last token; positions int64
+ *     [max_tokens]: its position in its request, 0 for those.
+ * lengths outside [0, M * page_size] are clamped; page numbers outside [0, P) in the table yield slot -1.  The rows of a table may share no page
+ * with each other if they are released through this call.  ws: vm_paged_plan_ws(N) bytes, 16-byte aligned.
+ * vm_paged_kv_write: k_pages[slot / page_size, h, slot % page_size, :] = k[t, h, :], v likewise; tokens whose slot lies outside
+ * [0, P * page_size) are skipped.  k, v: [T, Hkv, dh] with unit column stride, other strides in elements.  The slots of one call must differ.
+ * vm_paged_attention: one query token per row, o[n, h] = sum_j softmax_j(scale * q[n, h] . K_j) V_j over j < lengths[n] (clamped to M * page_size)
+ * of key head h / (Hq / Hkv); keys of pages outside [0, P) do not exist; no key at all: zeros.  dh a multiple of 8 up to 256, page_size a power of
+ * two from 16 on.  q: unit column stride; o: contiguous [N, Hq, dh].  ws: vm_paged_attention_ws(...) bytes, 16-byte aligned, NULL where it is 0. */
+size_t vm_paged_plan_ws(int N);
+int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int64_t ld_table, int N, int M, int32_t* free_pages, int32_t* ring,
+                  int P, int page_size, int64_t* slots, int64_t* positions, int max_tokens, int32_t* cu_tokens, int32_t* granted, void* ws,
+                  size_t ws_bytes, void* stream);
+int vm_paged_kv_write(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                      void* k_pages, void* v_pages, const int64_t* slots, int T, int Hkv, int dh, int P, int page_size, int dtype, void* stream);
+size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, int page_size, int dtype);
+int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                       int64_t ld_table, const int32_t* lengths, void* o, int N, int Hq, int Hkv, int dh, int P, int page_size, int M, float scale, int dtype,
+                       void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ log probabilities of given tokens (csrc/token_logprobs.hip)
+ * Row r of the logits (bf16 / fp32, unit column stride) starts at (r / inner) * ld_outer + (r % inner) * ld_inner elements.  With
+ * z = log sum exp(x), p = exp(x - z):
+ *   logp[r] = x_t - z (0 for a target < 0, NaN for a target >= V), entropy[r] = -sum_c p_c log p_c,
+ *   stats [R, 2] = (max x, z - max x): what the backward pass needs of the row,
+ *   top_ids / top_logp [R, top]: the ``top`` (<= VM_MAX_TOP_LOGPROBS) largest logits of the row, largest first, equal ones by ascending column.
+ * Logits of -inf are columns that do not exist (p = 0); a row of nothing else gives -inf, entropy 0, gradient 0.  The per-token scores of
+ * hf:generation/utils.py compute_transition_scores and the policy term of ref:vilmedic/blocks/rl/SCST.py:14-45.
+ * vm_token_logprobs_bwd: dlogits (rows ld_dlogits apart, the logits' type) = d/dx sum_r (g_logp logp + g_entropy entropy + sum_k g_top top_logp);
+ * each of the three gradients may be NULL (= 0). */
+#define VM_MAX_TOP_LOGPROBS 32
+int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top, float* logp,
+                          float* entropy, float* stats, float* top_logp, int64_t* top_ids, int dtype, void* stream);
+int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
+                          const float* stats, const float* entropy, const int64_t* top_ids, const float* g_logp, const float* g_entropy, const float* g_top,
+                          void* dlogits, int64_t ld_dlogits, int dtype, void* stream);
+
 /* ---- image input pipeline on the device (replaces, for decoded uint8 HWC images resident in HBM, the PIL / torchvision
    chain of vilmedic/datasets/base/ImageDataset.py:96-108: Resize -> RandomCrop -> RandomHorizontalFlip -> ToTensor ->
    Normalize for training (resize > 0), Resize((crop,crop)) -> ToTensor -> Normalize for evaluation (resize == 0)).

@@ -13,8 +13,10 @@ Design notes
 import bisect
 import contextlib
 import ctypes as C
+import functools
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -1209,3 +1211,199 @@ def lm_logits_f32(h2, emb_sh, bias, V):
         torch.empty(M, (V + 3) // 4 * 4, dtype=torch.float32, device=h2.device)
     gemm(h2, 0, emb_sh, 0, out, M, V, D, bias=bias)
     return out[:, :V]
+
+
+# ----------------------------------------------------------------------------- paged key-value cache (serving)
+# One decode step of a ragged batch:  paged_plan (pages, slots, positions of the new tokens) -> paged_kv_write -> paged_attention, the last two once
+# per layer.  The cache of a layer is k_pages, v_pages [P, Hkv, page_size, dh]; block_table int32 [N, M] and lengths int32 [N] are shared by
+# the layers.  Nothing here reads device data on the host, so a whole step can be captured into a HIP graph.  Scratch memory is taken from torch's
+# allocator inside the call: two captured graphs, or two streams, never share it.
+MAX_TOP_LOGPROBS = 32
+_DT = {torch.float32: VM_F32, BF16: VM_BF16}
+
+
+def _on_device_of(fn):
+    """launch on the device (and its current stream) that the call's tensors live on, whichever device is current"""
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        t = args[0] if args else next((x for x in kw.values() if isinstance(x, torch.Tensor)), None)
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return fn(*args, **kw)
+        return fn(*args, **kw)
+    return call
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _need_inference(name, *tensors):
+    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), f"{name} has no backward pass: call it under torch.no_grad()")
+
+
+def _need_same_device(name, first, *others):
+    for t in others:
+        _need(t.device == first.device, f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
+
+
+@_on_device_of
+def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_size, max_tokens):
+    """Admit, grow and release the requests of a paged cache on the device (vm_paged_plan).
+
+    ``lengths`` int32 [N], ``block_table`` int32 [N, M], ``free_pages`` int32 [P] (a ring of free page numbers) and ``free_ring`` int32 [2] =
+    (head, count) are updated in place; ``new_tokens`` int32 [N]: > 0 tokens to append to the row, 0 nothing, < 0 release the row (its pages can be
+    taken from the next call on).  A row whose tokens fit neither its table row, nor ``max_tokens`` (packed, all rows), nor the free pages is
+    refused: nothing about it changes.
+    -> (slots int64 [max_tokens], positions int64 [max_tokens], cu_tokens int32 [N + 1], granted int32 [N]): where the packed new tokens go
+    (-1: nowhere), their positions in their requests, the packed offsets of the rows, and the tokens each row was given."""
+    for name, t, nd in (("lengths", lengths, 1), ("new_tokens", new_tokens, 1), ("block_table", block_table, 2), ("free_pages", free_pages, 1),
+                        ("free_ring", free_ring, 1)):
+        _need(t.dim() == nd and t.dtype == torch.int32, f"paged_plan: {name} must be an int32 tensor of {nd} dimension(s), got {tuple(t.shape)} {t.dtype}")
+    N, M = block_table.shape
+    page_size, max_tokens = int(page_size), int(max_tokens)
+    _need(lengths.shape[0] == N and new_tokens.shape[0] == N, f"paged_plan: lengths and new_tokens must have the table's {N} rows")
+    _need(lengths.is_contiguous() and new_tokens.is_contiguous() and free_pages.is_contiguous() and free_ring.is_contiguous() and
+          (M < 2 or block_table.stride(1) == 1) and (N < 2 or block_table.stride(0) >= M), "paged_plan: the tensors must be contiguous (the table: its rows)")
+    _need(free_ring.shape[0] == 2, "paged_plan: free_ring must hold (head, count)")
+    _need(N > 0 and M > 0 and free_pages.shape[0] > 0 and page_size > 0, "paged_plan: at least one row, one column, one page and one token per page")
+    _need(0 <= max_tokens <= 1 << 30, f"paged_plan: max_tokens must lie between 0 and 2^30, got {max_tokens}")
+    _need(N * M < 1 << 31 and M * page_size < 1 << 31, "paged_plan: the table's size and M * page_size must stay below 2^31")
+    _need_same_device("paged_plan", lengths, new_tokens, block_table, free_pages, free_ring)
+    p = [ptr(t) for t in (lengths, new_tokens, block_table, free_pages, free_ring)]
+    dev = lengths.device
+    out = torch.empty(2, max_tokens, dtype=torch.int64, device=dev)
+    small = torch.empty(2 * N + 1, dtype=torch.int32, device=dev)
+    ws = torch.empty(lib().vm_paged_plan_ws(N), dtype=torch.uint8, device=dev)
+    slots, positions, cu, granted = out[0], out[1], small[:N + 1], small[N + 1:]
+    check(lib().vm_paged_plan(p[0], p[1], p[2], max(block_table.stride(0), M), N, M, p[3], p[4], free_pages.shape[0], page_size, ptr(slots), ptr(positions),
+                              max_tokens, ptr(cu), ptr(granted), ptr(ws), ws.numel(), stream()), "vm_paged_plan")
+    return slots, positions, cu, granted
+
+
+def _need_pages(name, k_pages, v_pages, other):
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, f"{name}: k_pages and v_pages must be [P, Hkv, page_size, dh], got "
+          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    _need(k_pages.dtype in _DT and k_pages.dtype == v_pages.dtype == other.dtype, f"{name}: one type, float32 or bfloat16, for the pages and what meets "
+          f"them, got {k_pages.dtype}, {v_pages.dtype} and {other.dtype}")
+    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), f"{name}: the pages must be contiguous")
+    P, H, s, dh = k_pages.shape
+    _need(P > 0 and H > 0 and 8 <= dh <= 256 and dh % 8 == 0, f"{name}: heads of a multiple of 8 columns up to 256 are supported, got {dh}")
+    _need(s >= 16 and s & (s - 1) == 0, f"{name}: page_size must be a power of two from 16 on, got {s}")
+    _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, f"{name}: the pages must start at a multiple of 16 bytes")
+
+
+@_on_device_of
+def paged_kv_write(k, v, k_pages, v_pages, slots):
+    """Write new tokens' keys and values ``k``, ``v`` [T, Hkv, dh] (unit column stride, any other strides: column slices of a fused projection are fine)
+    to ``slots`` int64 [T] of the pages; a slot outside [0, P * page_size) -- paged_plan's -1 -- writes nothing.  The slots of one call must differ
+    (of two equal ones either token's values may stay, piece by piece)."""
+    _need(k.dim() == 3 and k.shape == v.shape, f"paged_kv_write: k and v must be [T, Hkv, dh], got {tuple(k.shape)} and {tuple(v.shape)}")
+    _need(v.dtype == k.dtype, f"paged_kv_write: k and v must have one type, got {k.dtype} and {v.dtype}")
+    _need_pages("paged_kv_write", k_pages, v_pages, k)
+    P, H, s, dh = k_pages.shape
+    T = k.shape[0]
+    _need(tuple(k.shape[1:]) == (H, dh), f"paged_kv_write: the pages hold {H} heads of {dh} columns, k has {tuple(k.shape[1:])}")
+    _need(slots.dtype == torch.int64 and tuple(slots.shape) == (T,) and (T < 2 or slots.stride(0) == 1), "paged_kv_write: slots must be a contiguous int64 "
+          f"tensor of the {T} tokens, got {tuple(slots.shape)} {slots.dtype}")
+    _need(k.stride(2) == 1 and v.stride(2) == 1, "paged_kv_write: the columns of k and v must be contiguous")
+    _need_inference("paged_kv_write", k, v, k_pages, v_pages)
+    _need_same_device("paged_kv_write", k, v, k_pages, v_pages, slots)
+    if T == 0:
+        return
+    check(lib().vm_paged_kv_write(ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(k_pages), ptr(v_pages), ptr(slots), T, H, dh, P, s,
+                                  _DT[k.dtype], stream()), "vm_paged_kv_write")
+
+
+@_on_device_of
+def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
+    """Attention of one new token per row over its paged history: ``q`` [N, Hq, dh] (unit column stride; Hq a multiple of the pages' Hkv heads: query head h
+    reads key head h // (Hq / Hkv)), pages [P, Hkv, page_size, dh], ``block_table`` int32 [N, M], ``lengths`` int32 [N] (the new token's own key included,
+    if it is to see itself).  ``scale`` defaults to dh ** -0.5.  -> [N, Hq, dh] in q's type; a row of length 0 gives zeros, keys in pages that
+    do not exist (numbers outside [0, P)) are left out, stale values behind a row's length are never read into a result."""
+    _need(q.dim() == 3, f"paged_attention: q must be [N, Hq, dh], got {tuple(q.shape)}")
+    _need_pages("paged_attention", k_pages, v_pages, q)
+    P, H, s, dh = k_pages.shape
+    N, Hq = q.shape[0], q.shape[1]
+    _need(q.shape[2] == dh and Hq > 0 and Hq % H == 0, f"paged_attention: q {tuple(q.shape)} does not fit {H} key heads of {dh} columns")
+    _need(q.stride(2) == 1, "paged_attention: the columns of q must be contiguous")
+    _need(block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.shape[0] == N and block_table.shape[1] > 0 and
+          (block_table.shape[1] < 2 or block_table.stride(1) == 1) and (N < 2 or block_table.stride(0) >= block_table.shape[1]),
+          f"paged_attention: block_table must be int32 [{N}, M] with contiguous rows, got {tuple(block_table.shape)} {block_table.dtype}")
+    _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (N,) and (N < 2 or lengths.stride(0) == 1),
+          f"paged_attention: lengths must be a contiguous int32 tensor of {N} rows, got {tuple(lengths.shape)} {lengths.dtype}")
+    M = block_table.shape[1]
+    _need(M * s < 1 << 31 and N * Hq < 1 << 31, "paged_attention: M * page_size and N * Hq must stay below 2^31")
+    _need_inference("paged_attention", q, k_pages, v_pages)
+    _need_same_device("paged_attention", q, k_pages, v_pages, block_table, lengths)
+    p = [ptr(t) for t in (q, k_pages, v_pages, block_table, lengths)]
+    o = torch.empty(N, Hq, dh, dtype=q.dtype, device=q.device)
+    if N == 0:
+        return o
+    nws = lib().vm_paged_attention_ws(N, Hq, H, dh, M, s, _DT[q.dtype])
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    check(lib().vm_paged_attention(p[0], q.stride(0), q.stride(1), p[1], p[2], p[3], max(block_table.stride(0), M), p[4], ptr(o), N, Hq, H, dh, P, s, M,
+                                   dh ** -0.5 if scale is None else float(scale), _DT[q.dtype], ptr(ws), nws, stream()), "vm_paged_attention")
+    return o
+
+
+# ----------------------------------------------------------------------------- log probabilities of given tokens
+class TokenLogprobs(NamedTuple):
+    logp: torch.Tensor            # [...] fp32: log p(target); 0 where the target is negative
+    entropy: torch.Tensor         # [...] fp32: of the row's distribution
+    top_logp: torch.Tensor        # [..., top] fp32: the best alternatives, best first
+    top_ids: torch.Tensor         # [..., top] int64
+
+
+class TokenLogprobsFn(Fn):
+    """logits as a [A, B, V] view with unit column stride (rows A x B in order: a shifted slice of the decoder's logits needs no copy)"""
+
+    @staticmethod
+    def forward(ctx, x, targets, top, shape):
+        A, B, V = x.shape
+        logp, ent = (torch.empty(shape, dtype=torch.float32, device=x.device) for _ in range(2))
+        stats = torch.empty(A * B, 2, dtype=torch.float32, device=x.device)
+        best = torch.empty(*shape, top, dtype=torch.float32, device=x.device)
+        ids = torch.empty(*shape, top, dtype=torch.int64, device=x.device)
+        check(lib().vm_token_logprobs_fwd(ptr(x), x.stride(0), x.stride(1), B, ptr(targets), A * B, V, top, ptr(logp), ptr(ent), ptr(stats), ptr(best), ptr(ids),
+                                          _DT[x.dtype], stream()), "vm_token_logprobs_fwd")
+        ctx.save_for_backward(x, targets, stats, ent, ids)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return logp, ent, best, ids
+
+    @staticmethod
+    def backward(ctx, g_logp, g_ent, g_top, _g_ids):
+        x, targets, stats, ent, ids = ctx.saved_tensors
+        A, B, V = x.shape
+        ld = x.stride(1) if V <= x.stride(1) < V + 8 else V           # the logits' own padded rows, where they have such
+        dx = torch.empty(A * B, ld, dtype=x.dtype, device=x.device)
+        g = [t.float().contiguous() if t is not None else None for t in (g_logp, g_ent, g_top if ids.shape[-1] else None)]
+        with torch.cuda.device(x.device):
+            check(lib().vm_token_logprobs_bwd(ptr(x), x.stride(0), x.stride(1), B, ptr(targets), A * B, V, ids.shape[-1], ptr(stats), ptr(ent), ptr(ids), ptr(g[0]),
+                                              ptr(g[1]), ptr(g[2]), ptr(dx), ld, _DT[x.dtype], stream()), "vm_token_logprobs_bwd")
+        return dx.view(A, B, ld)[..., :V], None, None, None
+
+
+@_on_device_of
+def token_logprobs(logits, targets, top=0):
+    """Log probability of ``targets`` int64 [...] under softmax(``logits`` [..., V], float32 or bfloat16), the entropy of each distribution and its ``top``
+    (<= 32) most likely columns (largest first, equal logits by ascending column), differentiable with respect to the logits through all three.
+    A negative target is no token (logp 0, no gradient from it), one from V on gives NaN.  Columns at -inf (banned tokens, a top-k filter) have
+    probability 0 and gradient 0; a row of nothing else gives log probabilities -inf, entropy 0 and gradient 0.  Statistics are fp32 throughout.
+    -> TokenLogprobs(logp, entropy, top_logp, top_ids)"""
+    _need(logits.dtype in _DT, f"token_logprobs: logits must be float32 or bfloat16, got {logits.dtype}")
+    _need(logits.dim() >= 1 and targets.dtype == torch.int64 and targets.shape == logits.shape[:-1],
+          f"token_logprobs: targets must be int64 {tuple(logits.shape[:-1])}, got {tuple(targets.shape)} {targets.dtype}")
+    top, V, shape = int(top), logits.shape[-1], targets.shape
+    _need(V > 0 and 0 <= top <= min(V, MAX_TOP_LOGPROBS), f"token_logprobs: top must lie between 0 and min(V, {MAX_TOP_LOGPROBS}), got {top} (V = {V})")
+    _need(V < 1 << 30 and targets.numel() < 1 << 31, "token_logprobs: fewer than 2^30 columns and 2^31 rows are supported")
+    _need_same_device("token_logprobs", logits, targets)
+    x = logits if logits.dim() == 3 else logits[None] if logits.dim() == 2 else logits.reshape(1, -1, V)
+    if V > 1 and x.stride(2) != 1:
+        x = x.contiguous()
+    if targets.numel() == 0:
+        z = logits.float().sum(-1)
+        return TokenLogprobs(z, z.clone(), z.new_zeros(*shape, top), targets.new_zeros(*shape, top))
+    return TokenLogprobs(*TokenLogprobsFn.apply(x, targets.contiguous(), top, shape))
