@@ -2,70 +2,374 @@
 //   o[n, h] = sum_j softmax_j(scale * q[n, h] . K_j) V_j     over the keys j < lengths[n] of head h / (Hq / Hkv), key j in page block_table[n, j / s]
 // A key whose page number lies outside [0, P) does not exist, and no key at all leaves a row of zeros; what a page holds behind a row's length is
 // never multiplied (stale values, NaN included, do not reach the result).
+//
+// Every key and value is read once: the operator is bound by the bandwidth of the cache, and by the latency of one pass where that is short.  One
+// workgroup of four waves serves the (up to 16) query heads of one key head over one stretch of one row's keys; the waves take consecutive tiles of
+// the stretch and run an online softmax over them (running maximum m and sum l per query, base 2), so the cache is walked in one pass.
+//   * both products run on the matrix unit with the KEYS as the wide operand: S^T = K Q^T and O^T = V^T P^T.  A lane then owns ONE query (its
+//     column, lane % 16) throughout: the scores it gets are the probabilities it feeds back (same registers), its m, l and rescale factor are its
+//     own, and only the maximum crosses lanes (two swaps per tile).  With fewer than 16 queries the other columns idle; the unit is far from
+//     its limit all the same (a tile of 32 keys x 128 columns costs ~0.6 us of a SIMD's matrix time per 16 KB, 1 us of the chip's bandwidth share).
+//   * K goes straight from memory into the matrix unit's registers (16 B a lane, no LDS): the order in which the contraction visits the columns is
+//     free as long as Q uses the same.  V is needed with the keys along the contraction, 8 (bf16) or 4 (fp32) keys per lane; its rows are loaded
+//     as they lie, W consecutive columns a lane, and a pair of keys is interleaved with one byte permute (bf16; fp32 needs none).
+//   * the head's run inside a page is contiguous and a 16-key subtile never leaves its page, so a subtile's address is one scalar base (its page
+//     number, fetched 64 subtiles ahead into a register) plus offsets that no lane ever recomputes.
+//   * long rows are split over workgroups (``splits``); partial (m, l, O) in fp32 go to a workspace and a second launch joins them.  Each row is
+//     split by its OWN length, so the table's width decides only how many workgroups start.
 #include "common.h"
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 struct PagedAttnArgs {
     const void* q; int64_t q_row, q_head; const void* k; const void* v; const int32_t* table; int64_t ld_table; const int32_t* lengths; void* o;
-    int N, Hq, Hk, G, dh, P, s, M; float scale_log2;
+    float* part_o; float* part_ml; int N, Hq, Hk, G, qblocks, dh, P, shift, M, splits; float scale_log2;
 };
-template <typename T> __device__ __forceinline__ float ld1(const T* p);
-template <> __device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
-template <> __device__ __forceinline__ float ld1<bf16_t>(const bf16_t* p) { return bf16_to_f32(*p); }
-__device__ __forceinline__ void st1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void st1(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+#define PA_WAVES 4
+__device__ __forceinline__ void pa_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void pa_store(bf16_t* p, float v) { *p = f32_to_bf16(v); }
 
-// one wave per (row, query head): a lane scores one key, then the lanes split the head's columns
-template <typename T>
-__global__ __launch_bounds__(64) void paged_attention_kernel(const PagedAttnArgs p) {
-    __shared__ float qs[256];
-    __shared__ float ps[64];
-    __shared__ int64_t at[64];
-    const int lane = threadIdx.x, n = blockIdx.x / p.Hq, h = blockIdx.x - n * p.Hq, kv = h / p.G;
-    const T* q = (const T*)p.q + n * p.q_row + h * p.q_head;
-    for (int d = lane; d < p.dh; d += 64) qs[d] = ld1(q + d) * p.scale_log2;
-    int64_t len = p.lengths[n];
-    const int64_t cap = (int64_t)p.M * p.s;
-    len = len < 0 ? 0 : (len > cap ? cap : len);
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    __syncthreads();
-    for (int64_t j0 = 0; j0 < len; j0 += 64) {
-        const int64_t j = j0 + lane;
-        int64_t row = -1;
-        float sc = -INFINITY;
-        if (j < len) {
-            const int page = p.table[n * p.ld_table + j / p.s];
-            if (page >= 0 && page < p.P) {
-                row = (((int64_t)page * p.Hk + kv) * p.s + j % p.s) * p.dh;
-                const T* k = (const T*)p.k + row;
-                sc = 0.f;
-                for (int d = 0; d < p.dh; ++d) sc = fmaf(qs[d], ld1(k + d), sc);
+__device__ __forceinline__ float pa_col_max(float v) {          // over the four lanes of a column (lane ^ 16, lane ^ 32)
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float pa_col_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// W columns of V per lane (16 W >= dh), SUB 16-key subtiles per tile
+template <typename T, int W> struct PaTile;
+
+template <int W> struct PaTile<bf16_t, W> {
+    static constexpr int SUB = 2, KC = (16 * W + 31) / 32;       // K fragments of 32 columns: 8 per lane
+    static constexpr int VD = W / 2;                              // dwords of V per lane and key
+    uint4 q[KC];
+    uint4 k[SUB][KC];
+    uint32_t v[SUB][4][VD];
+    __device__ __forceinline__ void load_q(const bf16_t* row, int g, int dh, bool live) {      // any stride and alignment: element loads
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = c * 32 + g * 8 + 2 * i;
+                w[i] = live && d < dh ? (uint32_t)row[d] | ((uint32_t)row[d + 1] << 16) : 0u;
             }
+            q[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        const float mn = fmaxf(m, wave_max(sc));
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float e = exp2f(sc - base), f = exp2f(m - base);
-        l = l * f + wave_sum(e);
-        m = mn;
-        __syncthreads();
-        ps[lane] = e; at[lane] = row;
-        __syncthreads();
+    }
+    // base: the subtile's first key row; lane offsets in elements (r = lane % 16, g = lane / 16)
+    __device__ __forceinline__ void load_k(int u, const bf16_t* base, int r, int g, int dh) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            k[u][c] = make_uint4(0, 0, 0, 0);
+            if (c * 32 + g * 8 < dh) k[u][c] = *reinterpret_cast<const uint4*>(base + r * dh + g * 8 + c * 32);
+        }
+    }
+    __device__ __forceinline__ void load_v(int u, const bf16_t* base, int r, int g, int dh) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int d = lane + 64 * i;
-            if (d < p.dh) {
-                float a = acc[i] * f;
-                for (int u = 0; u < 64; ++u) if (at[u] >= 0) a = fmaf(ps[u], ld1((const T*)p.v + at[u] + d), a);
-                acc[i] = a;
+            const bf16_t* p = base + (g * 4 + i) * dh + r * W;
+#pragma unroll
+            for (int d = 0; d < VD; ++d) v[u][i][d] = 0;
+            if constexpr (VD == 1) { if (r * W < dh) v[u][i][0] = *reinterpret_cast<const uint32_t*>(p); }
+            else if constexpr (VD == 2) { if (r * W < dh) { const uint2 x = *reinterpret_cast<const uint2*>(p); v[u][i][0] = x.x; v[u][i][1] = x.y; } }
+            else {
+#pragma unroll
+                for (int d = 0; d < VD; d += 4) {                 // (16 columns a lane: a row may end behind the first eight)
+                    if (r * W + 2 * d < dh) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(p + 2 * d);
+                        v[u][i][d] = x.x; v[u][i][d + 1] = x.y; v[u][i][d + 2] = x.z; v[u][i][d + 3] = x.w;
+                    }
+                }
             }
         }
     }
-    T* o = (T*)p.o + ((int64_t)n * p.Hq + h) * p.dh;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    __device__ __forceinline__ void drop_v(int u, int i, bool ok) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (lane + 64 * i < p.dh) st1(o + lane + 64 * i, l == 0.f ? 0.f : acc[i] * inv);
+        for (int d = 0; d < VD; ++d) v[u][i][d] = ok ? v[u][i][d] : 0u;
+    }
+    __device__ __forceinline__ void scores(float4_t (&s)[SUB]) const {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[u][c]), __builtin_bit_cast(bf16x8_t, q[c]), s[u], 0, 0, 0);
+        }
+    }
+    // O^T += V^T P^T.  A probability goes in as two bf16 parts, hi (truncated) + lo: one bf16 would cost 2^-9 of every probability; the second
+    // product is free next to the loads.  hi is taken from p (1 - 2^-9), so that lo is positive wherever p is: an infinite V then stays infinite
+    // (0 * inf would make it NaN); what is left out is below 2^-16 of p.
+    __device__ __forceinline__ void accumulate(const float4_t (&p)[SUB], float4_t (&o)[W]) const {
+        uint4 hi, lo;
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = p[e >> 1][2 * (e & 1)], b = p[e >> 1][2 * (e & 1) + 1];
+            const uint32_t ah = __float_as_uint(a * (1.f - 1.f / 512)) & 0xffff0000u, bh = __float_as_uint(b * (1.f - 1.f / 512)) & 0xffff0000u;
+            h[e] = (ah >> 16) | bh;
+            l[e] = pack_bf16x2(a - __uint_as_float(ah), b - __uint_as_float(bh));
+        }
+        hi = make_uint4(h[0], h[1], h[2], h[3]); lo = make_uint4(l[0], l[1], l[2], l[3]);
+        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, hi), pl = __builtin_bit_cast(bf16x8_t, lo);
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {                            // the dword holds columns 2 d (low half) and 2 d + 1
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = v[e >> 1][2 * (e & 1)][d], y = v[e >> 1][2 * (e & 1) + 1][d];
+                a[e] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                b[e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+            }
+            const bf16x8_t va = __builtin_bit_cast(bf16x8_t, make_uint4(a[0], a[1], a[2], a[3])), vb = __builtin_bit_cast(bf16x8_t, make_uint4(b[0], b[1], b[2], b[3]));
+            o[2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[2 * d], 0, 0, 0);
+            o[2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, ph, o[2 * d + 1], 0, 0, 0);
+            o[2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pl, o[2 * d], 0, 0, 0);
+            o[2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, pl, o[2 * d + 1], 0, 0, 0);
+        }
+    }
+};
+
+// fp32: exact products on the f32 matrix instruction (4 columns / 4 keys per step; element j of a lane's 16 B feeds step j)
+template <int W> struct PaTile<float, W> {
+    static constexpr int SUB = W <= 4 ? 2 : 1, KC = W;
+    float4_t q[KC];
+    float4_t k[SUB][KC];
+    float v[SUB][4][W];
+    __device__ __forceinline__ void load_q(const float* row, int g, int dh, bool live) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[c][i] = live && c * 16 + g * 4 + i < dh ? row[c * 16 + g * 4 + i] : 0.f;
+    }
+    __device__ __forceinline__ void load_k(int u, const float* base, int r, int g, int dh) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            k[u][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+            if (c * 16 + g * 4 < dh) k[u][c] = *reinterpret_cast<const float4_t*>(base + r * dh + g * 4 + c * 16);
+        }
+    }
+    __device__ __forceinline__ void load_v(int u, const float* base, int r, int g, int dh) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* p = base + (g * 4 + i) * dh + r * W;
+#pragma unroll
+            for (int d = 0; d < W; ++d) v[u][i][d] = 0.f;
+            if constexpr (W == 2) { if (r * W < dh) { const float2 x = *reinterpret_cast<const float2*>(p); v[u][i][0] = x.x; v[u][i][1] = x.y; } }
+            else {
+#pragma unroll
+                for (int d = 0; d < W; d += 4) {
+                    if (r * W + d < dh) {
+                        const float4_t x = *reinterpret_cast<const float4_t*>(p + d);
+                        v[u][i][d] = x[0]; v[u][i][d + 1] = x[1]; v[u][i][d + 2] = x[2]; v[u][i][d + 3] = x[3];
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void drop_v(int u, int i, bool ok) {
+#pragma unroll
+        for (int d = 0; d < W; ++d) v[u][i][d] = ok ? v[u][i][d] : 0.f;
+    }
+    __device__ __forceinline__ void scores(float4_t (&s)[SUB]) const {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u][c][i], q[c][i], s[u], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void accumulate(const float4_t (&p)[SUB], float4_t (&o)[W]) const {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < W; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u][i][d], p[u][i], o[d], 0, 0, 0);
+    }
+};
+
+// tiles [t0, t1) of a row for (wave) part ``w`` of ``parts``
+__device__ __forceinline__ void pa_range(int tiles, int parts, int w, int& t0, int& t1) {
+    const int per = (tiles + parts - 1) / parts;
+    t0 = min(w * per, tiles);
+    t1 = min(t0 + per, tiles);
+}
+template <typename T, int W> __host__ __device__ constexpr int pa_tile_keys() { return 16 * PaTile<T, W>::SUB; }
+
+template <typename T, int W>
+__global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const PagedAttnArgs p) {
+    extern __shared__ __attribute__((aligned(16))) float pa_sm[];      // [waves][16][2] (m, l) | [waves][queries][dh] O
+    constexpr int SUB = PaTile<T, W>::SUB, TK = 16 * SUB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    int b = blockIdx.x;
+    const int split = b % p.splits; b /= p.splits;
+    const int qb = b % p.qblocks; b /= p.qblocks;
+    const int kv = b % p.Hk, n = b / p.Hk;
+    const int h0 = kv * p.G + qb * 16, nq = min(16, p.G - qb * 16);    // this workgroup's query heads
+    const int cap = p.M << p.shift;
+    const int len = min(max(p.lengths[n], 0), cap), tiles = (len + TK - 1) / TK;
+    int t0, t1;
+    pa_range(tiles, p.splits * PA_WAVES, split * PA_WAVES, t0, t1);
+    const bool only = p.splits == 1;
+    if (t0 >= t1 && !only) return;                                    // (workgroup-uniform; the join counts the stretches by the same rule)
+    pa_range(tiles, p.splits * PA_WAVES, split * PA_WAVES + wave, t0, t1);
+    PaTile<T, W> x;
+    x.load_q((const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, p.dh, r < nq);
+    float m = -INFINITY, l = 0.f;
+    float4_t o[W];
+#pragma unroll
+    for (int d = 0; d < W; ++d) o[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const int32_t* row = p.table + n * p.ld_table;
+    const int64_t head = (int64_t)kv << p.shift, page_rows = (int64_t)p.Hk << p.shift;
+    const int mask = (1 << p.shift) - 1;
+    int pages = 0;
+    for (int t = t0; t < t1; ++t) {
+        const int ahead = (t - t0) * SUB & 63;                        // page numbers of the next 64 subtiles, one per lane
+        if (ahead == 0) {
+            const int key = t * TK + lane * 16;
+            pages = key < len ? row[key >> p.shift] : -1;
+        }
+        bool good[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const int page = __builtin_amdgcn_readlane(pages, ahead + u);
+            good[u] = page >= 0 && page < p.P;
+            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + ((t * TK + u * 16) & mask)) * p.dh;
+            x.load_k(u, (const T*)p.k + at, r, g, p.dh);
+            x.load_v(u, (const T*)p.v + at, r, g, p.dh);
+        }
+        bool whole = (t + 1) * TK <= len;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) whole = whole && good[u];
+        float4_t s[SUB];
+        x.scores(s);
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = s[u][i] * p.scale_log2;
+                if (!whole) {
+                    const bool ok = good[u] && t * TK + u * 16 + g * 4 + i < len;
+                    v = ok ? v : -INFINITY;
+                    x.drop_v(u, i, ok);
+                }
+                s[u][i] = v;
+                mx = fmaxf(mx, v);
+            }
+        mx = pa_col_max(mx);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float f = __builtin_amdgcn_exp2f(m - base);             // 0 the first time (m = -inf)
+        if (__any(mx > m)) {
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < W; ++d) o[d] *= f;
+        }
+        m = mx;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - base); l += s[u][i]; }
+        x.accumulate(s, o);
+    }
+    l = pa_col_sum(l);
+    float* ml = pa_sm + wave * 32;
+    float* so = pa_sm + PA_WAVES * 32 + wave * nq * p.dh;
+    if (g == 0) { ml[2 * r] = m; ml[2 * r + 1] = l; }
+    if (r < nq) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < W; ++d) {
+                const int c = (g * 4 + i) * W + d;
+                if (c < p.dh) so[r * p.dh + c] = o[d][i];
+            }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nq * p.dh; e += 64 * PA_WAVES) {
+        const int qi = e / p.dh, c = e - qi * p.dh;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; ++w) mm = fmaxf(mm, pa_sm[w * 32 + 2 * qi]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        float acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(pa_sm[w * 32 + 2 * qi] - base);
+            acc = fmaf(f, pa_sm[PA_WAVES * 32 + (w * nq + qi) * p.dh + c], acc);
+            sum = fmaf(f, pa_sm[w * 32 + 2 * qi + 1], sum);
+        }
+        const int64_t out = (int64_t)n * p.Hq + h0 + qi;
+        if (only) {
+            pa_store((T*)p.o + out * p.dh + c, sum == 0.f ? 0.f : acc / sum);
+        } else {
+            p.part_o[(out * p.splits + split) * p.dh + c] = acc;
+            if (c == 0) { p.part_ml[2 * (out * p.splits + split)] = mm; p.part_ml[2 * (out * p.splits + split) + 1] = sum; }
+        }
+    }
 }
 
-extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, int page_size, int dtype) { return 0; }
+// one workgroup per (row, query head): the stretches' partial results, rescaled to their common maximum
+template <typename T>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttnArgs p, int tile_keys) {
+    const int64_t out = blockIdx.x;
+    const int n = blockIdx.x / p.Hq;
+    const int len = min(max(p.lengths[n], 0), p.M << p.shift), tiles = (len + tile_keys - 1) / tile_keys;
+    const int per = (tiles + p.splits * PA_WAVES - 1) / (p.splits * PA_WAVES), used = per ? (tiles + per * PA_WAVES - 1) / (per * PA_WAVES) : 0;
+    const float* ml = p.part_ml + 2 * out * p.splits;
+    float m = -INFINITY;
+    for (int s = 0; s < used; ++s) m = fmaxf(m, ml[2 * s]);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int c = threadIdx.x; c < p.dh; c += 256) {
+        float acc = 0.f, sum = 0.f;
+        for (int s = 0; s < used; ++s) {
+            const float f = __builtin_amdgcn_exp2f(ml[2 * s] - base);
+            acc = fmaf(f, p.part_o[(out * p.splits + s) * p.dh + c], acc);
+            sum = fmaf(f, ml[2 * s + 1], sum);
+        }
+        pa_store((T*)p.o + out * p.dh + c, sum == 0.f ? 0.f : acc / sum);
+    }
+}
+
+// how many workgroups share a row's keys
+static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
+    const int64_t blocks = (int64_t)N * Hkv * ((Hq / Hkv + 15) / 16);
+    const int64_t keys = (int64_t)M * page_size, most = (keys + 511) / 512;
+    int64_t s = (2048 + blocks - 1) / blocks;
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s);
+}
+extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, int page_size, int dtype) {
+    (void)dtype;
+    if (N <= 0 || Hq <= 0 || Hkv <= 0 || M <= 0 || page_size <= 0 || dh <= 0 || Hq % Hkv) return 0;
+    const int s = pa_splits(N, Hq, Hkv, M, page_size);
+    return s == 1 ? 0 : (size_t)N * Hq * s * (dh + 2) * sizeof(float);
+}
+
+template <typename T, int W>
+static void pa_launch(const PagedAttnArgs& a, hipStream_t s) {
+    const int nq = a.G < 16 ? a.G : 16;
+    const size_t lds = sizeof(float) * (PA_WAVES * 32 + (size_t)PA_WAVES * nq * a.dh);
+    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * PA_WAVES), lds, s, a);
+    if (a.splits > 1) hipLaunchKernelGGL(paged_attention_join_kernel<T>, dim3(a.N * a.Hq), dim3(256), 0, s, a, pa_tile_keys<T, W>());
+}
+template <typename T>
+static void pa_launch_w(const PagedAttnArgs& a, hipStream_t s) {
+    if (a.dh <= 32) pa_launch<T, 2>(a, s);
+    else if (a.dh <= 64) pa_launch<T, 4>(a, s);
+    else if (a.dh <= 128) pa_launch<T, 8>(a, s);
+    else pa_launch<T, 16>(a, s);
+}
 
 extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages,
                                   const int32_t* block_table, int64_t ld_table, const int32_t* lengths, void* o, int N, int Hq, int Hkv, int dh, int P,
@@ -73,16 +377,20 @@ extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q
     VM_REQUIRE(q && k_pages && v_pages && block_table && lengths && o, "vm_paged_attention: null pointer");
     VM_REQUIRE(N > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && P > 0 && M > 0 && ld_table >= M, "vm_paged_attention: bad shape");
     VM_REQUIRE(dh >= 8 && dh <= 256 && dh % 8 == 0, "vm_paged_attention: dh = %d: a multiple of 8 up to 256 is required", dh);
-    VM_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0 && (int64_t)M * page_size < (1ll << 31),
-               "vm_paged_attention: page_size must be a power of two from 16 on, M * page_size below 2^31");
+    VM_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0 && (int64_t)M * page_size < (1ll << 31) - 2048,
+               "vm_paged_attention: page_size must be a power of two from 16 on, M * page_size below 2^31 - 2048");
     VM_REQUIRE(dtype == VM_F32 || dtype == VM_BF16, "vm_paged_attention: dtype must be VM_F32 or VM_BF16");
     VM_REQUIRE(((uintptr_t)k_pages % 16) == 0 && ((uintptr_t)v_pages % 16) == 0, "vm_paged_attention: pages must be 16-byte aligned");
-    VM_REQUIRE((int64_t)N * Hq < (1ll << 31), "vm_paged_attention: N * Hq must stay below 2^31");
-    PagedAttnArgs a = {q, q_row_stride, q_head_stride, k_pages, v_pages, block_table, ld_table, lengths, o, N, Hq, Hkv, Hq / Hkv, dh, P, page_size, M,
+    const int splits = pa_splits(N, Hq, Hkv, M, page_size), qblocks = (Hq / Hkv + 15) / 16;
+    VM_REQUIRE((int64_t)N * Hq < (1ll << 31) && (int64_t)N * Hkv * qblocks * splits < (1ll << 31), "vm_paged_attention: too many rows x heads");
+    const size_t need = vm_paged_attention_ws(N, Hq, Hkv, dh, M, page_size, dtype);
+    VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_attention: 16-byte aligned workspace of %zu bytes required", need);
+    PagedAttnArgs a = {q, q_row_stride, q_head_stride, k_pages, v_pages, block_table, ld_table, lengths, o, (float*)ws,
+                       (float*)ws + (size_t)N * Hq * splits * dh, N, Hq, Hkv, Hq / Hkv, qblocks, dh, P, __builtin_ctz(page_size), M, splits,
                        scale * 1.4426950408889634f};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_ATTN, 0.0, s, "paged_attn_n%d_h%d_k%d_d%d", N, Hq, Hkv, dh);
-    if (dtype == VM_F32) hipLaunchKernelGGL(paged_attention_kernel<float>, dim3(N * Hq), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(paged_attention_kernel<bf16_t>, dim3(N * Hq), dim3(64), 0, s, a);
+    if (dtype == VM_F32) pa_launch_w<float>(a, s);
+    else pa_launch_w<bf16_t>(a, s);
     return vm_check_launch("vm_paged_attention");
 }

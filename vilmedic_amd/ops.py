@@ -1334,7 +1334,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
     _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (N,) and (N < 2 or lengths.stride(0) == 1),
           f"paged_attention: lengths must be a contiguous int32 tensor of {N} rows, got {tuple(lengths.shape)} {lengths.dtype}")
     M = block_table.shape[1]
-    _need(M * s < 1 << 31 and N * Hq < 1 << 31, "paged_attention: M * page_size and N * Hq must stay below 2^31")
+    _need(M * s < (1 << 31) - 2048 and N * Hq < 1 << 31, "paged_attention: M * page_size must stay below 2^31 - 2048, N * Hq below 2^31")
     _need_inference("paged_attention", q, k_pages, v_pages)
     _need_same_device("paged_attention", q, k_pages, v_pages, block_table, lengths)
     p = [ptr(t) for t in (q, k_pages, v_pages, block_table, lengths)]
