@@ -318,25 +318,46 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const Pa
     }
 }
 
-// one workgroup per (row, query head): the stretches' partial results, rescaled to their common maximum
+// one workgroup per (row, query head): the stretches' partial results, rescaled to their common maximum.  The stretches' weights go to LDS first (one
+// trip to memory for all of them), then the workgroup's groups of dh / 4 threads walk every groups-th stretch, 16 B a thread, and are added in LDS.
+#define PA_MAX_SPLITS 2048
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttnArgs p, int tile_keys) {
+    __shared__ float weight[PA_MAX_SPLITS];
+    __shared__ float4_t sums[256];
+    __shared__ float red[8];
     const int64_t out = blockIdx.x;
-    const int n = blockIdx.x / p.Hq;
+    const int n = blockIdx.x / p.Hq, tid = threadIdx.x;
     const int len = min(max(p.lengths[n], 0), p.M << p.shift), tiles = (len + tile_keys - 1) / tile_keys;
     const int per = (tiles + p.splits * PA_WAVES - 1) / (p.splits * PA_WAVES), used = per ? (tiles + per * PA_WAVES - 1) / (per * PA_WAVES) : 0;
-    const float* ml = p.part_ml + 2 * out * p.splits;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out * p.splits;
     float m = -INFINITY;
-    for (int s = 0; s < used; ++s) m = fmaxf(m, ml[2 * s]);
+    for (int s = tid; s < used; s += 256) m = fmaxf(m, ml[s].x);
+    m = wave_max(m);
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base = m == -INFINITY ? 0.f : m;
-    for (int c = threadIdx.x; c < p.dh; c += 256) {
-        float acc = 0.f, sum = 0.f;
-        for (int s = 0; s < used; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-            acc = fmaf(f, p.part_o[(out * p.splits + s) * p.dh + c], acc);
-            sum = fmaf(f, ml[2 * s + 1], sum);
-        }
-        pa_store((T*)p.o + out * p.dh + c, sum == 0.f ? 0.f : acc / sum);
+    float l = 0.f;
+    for (int s = tid; s < used; s += 256) { const float2 x = ml[s]; const float f = __builtin_amdgcn_exp2f(x.x - base); weight[s] = f; l = fmaf(f, x.y, l); }
+    l = wave_sum(l);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    const int lanes = p.dh / 4, groups = 256 / lanes, grp = tid / lanes, c = tid - grp * lanes;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    if (grp < groups) {
+        const float* po = p.part_o + out * p.splits * p.dh + 4 * c;
+#pragma unroll 4
+        for (int s = grp; s < used; s += groups) acc += weight[s] * *reinterpret_cast<const float4_t*>(po + (int64_t)s * p.dh);
+    }
+    sums[tid] = acc;
+    __syncthreads();
+    if (grp == 0) {
+        for (int j = 1; j < groups; ++j) acc += sums[j * lanes + c];
+        T* o = (T*)p.o + out * p.dh + 4 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pa_store(o + i, l == 0.f ? 0.f : acc[i] / l);
     }
 }
 
@@ -346,6 +367,7 @@ static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
     const int64_t keys = (int64_t)M * page_size, most = (keys + 511) / 512;
     int64_t s = (2048 + blocks - 1) / blocks;
     if (s > most) s = most;
+    if (s > PA_MAX_SPLITS) s = PA_MAX_SPLITS;
     return (int)(s < 1 ? 1 : s);
 }
 extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, int page_size, int dtype) {

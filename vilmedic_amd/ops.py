@@ -1218,8 +1218,12 @@ def lm_logits_f32(h2, emb_sh, bias, V):
 # per layer.  The cache of a layer is k_pages, v_pages [P, Hkv, page_size, dh]; block_table int32 [N, M] and lengths int32 [N] are shared by
 # the layers.  Nothing here reads device data on the host, so a whole step can be captured into a HIP graph.  Scratch memory is taken from torch's
 # allocator inside the call: two captured graphs, or two streams, never share it.
+#
+# A decode step makes these calls once per layer, and the kernels of a small batch take a few microseconds: the checks are plain comparisons (messages are
+# built only when one fails) and the sizes of scratch memory are remembered by their arguments.
 MAX_TOP_LOGPROBS = 32
 _DT = {torch.float32: VM_F32, BF16: VM_BF16}
+_I32, _I64 = torch.int32, torch.int64
 
 
 def _on_device_of(fn):
@@ -1227,25 +1231,34 @@ def _on_device_of(fn):
     @functools.wraps(fn)
     def call(*args, **kw):
         t = args[0] if args else next((x for x in kw.values() if isinstance(x, torch.Tensor)), None)
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
             with torch.cuda.device(t.device):
                 return fn(*args, **kw)
         return fn(*args, **kw)
     return call
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+def _refuse(name, why):
+    raise ValueError(f"{name}: {why}")
+
+
+def _desc(t):
+    return f"{tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}"
 
 
 def _need_inference(name, *tensors):
-    _need(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), f"{name} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        _refuse(name, "it has no backward pass: call it under torch.no_grad()")
 
 
-def _need_same_device(name, first, *others):
-    for t in others:
-        _need(t.device == first.device, f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
+@functools.lru_cache(maxsize=1024)
+def _plan_ws(N):
+    return lib().vm_paged_plan_ws(N)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_ws(N, Hq, H, dh, M, s, dt):
+    return lib().vm_paged_attention_ws(N, Hq, H, dh, M, s, dt)
 
 
 @_on_device_of
@@ -1258,40 +1271,65 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
     refused: nothing about it changes.
     -> (slots int64 [max_tokens], positions int64 [max_tokens], cu_tokens int32 [N + 1], granted int32 [N]): where the packed new tokens go
     (-1: nowhere), their positions in their requests, the packed offsets of the rows, and the tokens each row was given."""
-    for name, t, nd in (("lengths", lengths, 1), ("new_tokens", new_tokens, 1), ("block_table", block_table, 2), ("free_pages", free_pages, 1),
+    name = "paged_plan"
+    for what, t, nd in (("lengths", lengths, 1), ("new_tokens", new_tokens, 1), ("block_table", block_table, 2), ("free_pages", free_pages, 1),
                         ("free_ring", free_ring, 1)):
-        _need(t.dim() == nd and t.dtype == torch.int32, f"paged_plan: {name} must be an int32 tensor of {nd} dimension(s), got {tuple(t.shape)} {t.dtype}")
+        if t.dtype != _I32 or t.dim() != nd:
+            _refuse(name, f"{what} must be an int32 tensor of {nd} dimension(s), got {_desc(t)}")
+        if t.device != lengths.device:
+            _refuse(name, f"all tensors must be on one device, got {lengths.device} and {t.device}")
+        if nd == 1 and not t.is_contiguous():
+            _refuse(name, f"{what} must be contiguous")
     N, M = block_table.shape
+    P = free_pages.shape[0]
     page_size, max_tokens = int(page_size), int(max_tokens)
-    _need(lengths.shape[0] == N and new_tokens.shape[0] == N, f"paged_plan: lengths and new_tokens must have the table's {N} rows")
-    _need(lengths.is_contiguous() and new_tokens.is_contiguous() and free_pages.is_contiguous() and free_ring.is_contiguous() and
-          (M < 2 or block_table.stride(1) == 1) and (N < 2 or block_table.stride(0) >= M), "paged_plan: the tensors must be contiguous (the table: its rows)")
-    _need(free_ring.shape[0] == 2, "paged_plan: free_ring must hold (head, count)")
-    _need(N > 0 and M > 0 and free_pages.shape[0] > 0 and page_size > 0, "paged_plan: at least one row, one column, one page and one token per page")
-    _need(0 <= max_tokens <= 1 << 30, f"paged_plan: max_tokens must lie between 0 and 2^30, got {max_tokens}")
-    _need(N * M < 1 << 31 and M * page_size < 1 << 31, "paged_plan: the table's size and M * page_size must stay below 2^31")
-    _need_same_device("paged_plan", lengths, new_tokens, block_table, free_pages, free_ring)
+    ld = block_table.stride(0) if N > 1 else M
+    if lengths.shape[0] != N or new_tokens.shape[0] != N:
+        _refuse(name, f"lengths and new_tokens must have the table's {N} rows")
+    if (M > 1 and block_table.stride(1) != 1) or ld < M:
+        _refuse(name, f"the table's rows must be contiguous and apart, got {_desc(block_table)}")
+    if free_ring.shape[0] != 2:
+        _refuse(name, "free_ring must hold (head, count)")
+    if N < 1 or M < 1 or P < 1 or page_size < 1:
+        _refuse(name, "at least one row, one column, one page and one token per page")
+    if not 0 <= max_tokens <= 1 << 30:
+        _refuse(name, f"max_tokens must lie between 0 and 2^30, got {max_tokens}")
+    if N * M >= 1 << 31 or M * page_size >= 1 << 31:
+        _refuse(name, "the table's size and M * page_size must stay below 2^31")
     p = [ptr(t) for t in (lengths, new_tokens, block_table, free_pages, free_ring)]
-    dev = lengths.device
-    out = torch.empty(2, max_tokens, dtype=torch.int64, device=dev)
-    small = torch.empty(2 * N + 1, dtype=torch.int32, device=dev)
-    ws = torch.empty(lib().vm_paged_plan_ws(N), dtype=torch.uint8, device=dev)
-    slots, positions, cu, granted = out[0], out[1], small[:N + 1], small[N + 1:]
-    check(lib().vm_paged_plan(p[0], p[1], p[2], max(block_table.stride(0), M), N, M, p[3], p[4], free_pages.shape[0], page_size, ptr(slots), ptr(positions),
-                              max_tokens, ptr(cu), ptr(granted), ptr(ws), ws.numel(), stream()), "vm_paged_plan")
-    return slots, positions, cu, granted
+    # one allocation: slots | positions (8 bytes each) | scratch (16-byte rows) | cu_tokens | granted
+    nws = _plan_ws(N)
+    head = 16 * max_tokens
+    buf = torch.empty(head + nws + 4 * (2 * N + 1), dtype=torch.uint8, device=lengths.device)
+    at = buf.data_ptr()
+    cu = at + head + nws
+    check(lib().vm_paged_plan(p[0], p[1], p[2], ld, N, M, p[3], p[4], P, page_size, at if max_tokens else None, at + 8 * max_tokens if max_tokens else None,
+                              max_tokens, cu, cu + 4 * (N + 1), at + head, nws, stream()), name)
+    small = buf[head + nws:].view(_I32)
+    both = buf[:head].view(_I64)
+    return both[:max_tokens], both[max_tokens:], small[:N + 1], small[N + 1:]
 
 
-def _need_pages(name, k_pages, v_pages, other):
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape, f"{name}: k_pages and v_pages must be [P, Hkv, page_size, dh], got "
-          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    _need(k_pages.dtype in _DT and k_pages.dtype == v_pages.dtype == other.dtype, f"{name}: one type, float32 or bfloat16, for the pages and what meets "
-          f"them, got {k_pages.dtype}, {v_pages.dtype} and {other.dtype}")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), f"{name}: the pages must be contiguous")
-    P, H, s, dh = k_pages.shape
-    _need(P > 0 and H > 0 and 8 <= dh <= 256 and dh % 8 == 0, f"{name}: heads of a multiple of 8 columns up to 256 are supported, got {dh}")
-    _need(s >= 16 and s & (s - 1) == 0, f"{name}: page_size must be a power of two from 16 on, got {s}")
-    _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, f"{name}: the pages must start at a multiple of 16 bytes")
+def _check_pages(name, k_pages, v_pages, other):
+    """-> (P, Hkv, page_size, dh, dtype code)"""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
+        _refuse(name, f"k_pages and v_pages must be [P, Hkv, page_size, dh], got {_desc(k_pages)} and {_desc(v_pages)}")
+    dt = _DT.get(k_pages.dtype)
+    if dt is None or v_pages.dtype != k_pages.dtype or other.dtype != k_pages.dtype:
+        _refuse(name, f"one type, float32 or bfloat16, for the pages and what meets them, got {k_pages.dtype}, {v_pages.dtype} and {other.dtype}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _refuse(name, "the pages must be contiguous")
+    P, H, s, dh = shape
+    if P < 1 or H < 1 or not 8 <= dh <= 256 or dh % 8:
+        _refuse(name, f"at least one page and one head, heads of a multiple of 8 columns up to 256, got {tuple(shape)}")
+    if s < 16 or s & (s - 1):
+        _refuse(name, f"page_size must be a power of two from 16 on, got {s}")
+    if (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        _refuse(name, "the pages must start at a multiple of 16 bytes")
+    if k_pages.device != other.device or v_pages.device != other.device:
+        _refuse(name, f"all tensors must be on one device, got {other.device}, {k_pages.device} and {v_pages.device}")
+    return P, H, s, dh, dt
 
 
 @_on_device_of
@@ -1299,21 +1337,20 @@ def paged_kv_write(k, v, k_pages, v_pages, slots):
     """Write new tokens' keys and values ``k``, ``v`` [T, Hkv, dh] (unit column stride, any other strides: column slices of a fused projection are fine)
     to ``slots`` int64 [T] of the pages; a slot outside [0, P * page_size) -- paged_plan's -1 -- writes nothing.  The slots of one call must differ
     (of two equal ones either token's values may stay, piece by piece)."""
-    _need(k.dim() == 3 and k.shape == v.shape, f"paged_kv_write: k and v must be [T, Hkv, dh], got {tuple(k.shape)} and {tuple(v.shape)}")
-    _need(v.dtype == k.dtype, f"paged_kv_write: k and v must have one type, got {k.dtype} and {v.dtype}")
-    _need_pages("paged_kv_write", k_pages, v_pages, k)
-    P, H, s, dh = k_pages.shape
+    name = "paged_kv_write"
+    P, H, s, dh, dt = _check_pages(name, k_pages, v_pages, k)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != dh or v.dtype != k.dtype or v.device != k.device:
+        _refuse(name, f"k and v must be [T, {H}, {dh}] like the pages' heads, of one type, got {_desc(k)} and {_desc(v)}")
     T = k.shape[0]
-    _need(tuple(k.shape[1:]) == (H, dh), f"paged_kv_write: the pages hold {H} heads of {dh} columns, k has {tuple(k.shape[1:])}")
-    _need(slots.dtype == torch.int64 and tuple(slots.shape) == (T,) and (T < 2 or slots.stride(0) == 1), "paged_kv_write: slots must be a contiguous int64 "
-          f"tensor of the {T} tokens, got {tuple(slots.shape)} {slots.dtype}")
-    _need(k.stride(2) == 1 and v.stride(2) == 1, "paged_kv_write: the columns of k and v must be contiguous")
-    _need_inference("paged_kv_write", k, v, k_pages, v_pages)
-    _need_same_device("paged_kv_write", k, v, k_pages, v_pages, slots)
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
+        _refuse(name, f"the columns of k and v must be contiguous, got {_desc(k)} and {_desc(v)}")
+    if slots.dtype != _I64 or slots.dim() != 1 or slots.shape[0] != T or (T > 1 and slots.stride(0) != 1) or slots.device != k.device:
+        _refuse(name, f"slots must be a contiguous int64 tensor of the {T} tokens on their device, got {_desc(slots)}")
+    _need_inference(name, k, v, k_pages, v_pages)
     if T == 0:
         return
-    check(lib().vm_paged_kv_write(ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), ptr(k_pages), ptr(v_pages), ptr(slots), T, H, dh, P, s,
-                                  _DT[k.dtype], stream()), "vm_paged_kv_write")
+    check(lib().vm_paged_kv_write(ptr(k), ks[0], ks[1], ptr(v), vs[0], vs[1], ptr(k_pages), ptr(v_pages), ptr(slots), T, H, dh, P, s, dt, stream()), name)
 
 
 @_on_device_of
@@ -1322,29 +1359,32 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
     reads key head h // (Hq / Hkv)), pages [P, Hkv, page_size, dh], ``block_table`` int32 [N, M], ``lengths`` int32 [N] (the new token's own key included,
     if it is to see itself).  ``scale`` defaults to dh ** -0.5.  -> [N, Hq, dh] in q's type; a row of length 0 gives zeros, keys in pages that
     do not exist (numbers outside [0, P)) are left out, stale values behind a row's length are never read into a result."""
-    _need(q.dim() == 3, f"paged_attention: q must be [N, Hq, dh], got {tuple(q.shape)}")
-    _need_pages("paged_attention", k_pages, v_pages, q)
-    P, H, s, dh = k_pages.shape
-    N, Hq = q.shape[0], q.shape[1]
-    _need(q.shape[2] == dh and Hq > 0 and Hq % H == 0, f"paged_attention: q {tuple(q.shape)} does not fit {H} key heads of {dh} columns")
-    _need(q.stride(2) == 1, "paged_attention: the columns of q must be contiguous")
-    _need(block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.shape[0] == N and block_table.shape[1] > 0 and
-          (block_table.shape[1] < 2 or block_table.stride(1) == 1) and (N < 2 or block_table.stride(0) >= block_table.shape[1]),
-          f"paged_attention: block_table must be int32 [{N}, M] with contiguous rows, got {tuple(block_table.shape)} {block_table.dtype}")
-    _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (N,) and (N < 2 or lengths.stride(0) == 1),
-          f"paged_attention: lengths must be a contiguous int32 tensor of {N} rows, got {tuple(lengths.shape)} {lengths.dtype}")
+    name = "paged_attention"
+    P, H, s, dh, dt = _check_pages(name, k_pages, v_pages, q)
+    if q.dim() != 3 or q.shape[2] != dh or q.shape[1] < 1 or q.shape[1] % H:
+        _refuse(name, f"q must be [N, a multiple of {H} heads, {dh}], got {_desc(q)}")
+    N, Hq, _ = q.shape
+    qs = q.stride()
+    if qs[2] != 1:
+        _refuse(name, f"the columns of q must be contiguous, got {_desc(q)}")
+    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.shape[0] != N or block_table.shape[1] < 1 or block_table.device != q.device:
+        _refuse(name, f"block_table must be int32 [{N}, M] on q's device, got {_desc(block_table)}")
     M = block_table.shape[1]
-    _need(M * s < (1 << 31) - 2048 and N * Hq < 1 << 31, "paged_attention: M * page_size must stay below 2^31 - 2048, N * Hq below 2^31")
-    _need_inference("paged_attention", q, k_pages, v_pages)
-    _need_same_device("paged_attention", q, k_pages, v_pages, block_table, lengths)
-    p = [ptr(t) for t in (q, k_pages, v_pages, block_table, lengths)]
+    ld = block_table.stride(0) if N > 1 else M
+    if (M > 1 and block_table.stride(1) != 1) or ld < M:
+        _refuse(name, f"the table's rows must be contiguous and apart, got {_desc(block_table)}")
+    if lengths.dtype != _I32 or lengths.dim() != 1 or lengths.shape[0] != N or (N > 1 and lengths.stride(0) != 1) or lengths.device != q.device:
+        _refuse(name, f"lengths must be a contiguous int32 tensor of {N} rows on q's device, got {_desc(lengths)}")
+    if M * s >= (1 << 31) - 2048 or N * Hq >= 1 << 31:
+        _refuse(name, "M * page_size must stay below 2^31 - 2048, N * Hq below 2^31")
+    _need_inference(name, q, k_pages, v_pages)
     o = torch.empty(N, Hq, dh, dtype=q.dtype, device=q.device)
     if N == 0:
         return o
-    nws = lib().vm_paged_attention_ws(N, Hq, H, dh, M, s, _DT[q.dtype])
+    nws = _attention_ws(N, Hq, H, dh, M, s, dt)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    check(lib().vm_paged_attention(p[0], q.stride(0), q.stride(1), p[1], p[2], p[3], max(block_table.stride(0), M), p[4], ptr(o), N, Hq, H, dh, P, s, M,
-                                   dh ** -0.5 if scale is None else float(scale), _DT[q.dtype], ptr(ws), nws, stream()), "vm_paged_attention")
+    check(lib().vm_paged_attention(ptr(q), qs[0], qs[1], ptr(k_pages), ptr(v_pages), ptr(block_table), ld, ptr(lengths), ptr(o), N, Hq, H, dh, P, s, M,
+                                   dh ** -0.5 if scale is None else float(scale), dt, ptr(ws), nws, stream()), name)
     return o
 
 
@@ -1393,13 +1433,16 @@ def token_logprobs(logits, targets, top=0):
     A negative target is no token (logp 0, no gradient from it), one from V on gives NaN.  Columns at -inf (banned tokens, a top-k filter) have
     probability 0 and gradient 0; a row of nothing else gives log probabilities -inf, entropy 0 and gradient 0.  Statistics are fp32 throughout.
     -> TokenLogprobs(logp, entropy, top_logp, top_ids)"""
-    _need(logits.dtype in _DT, f"token_logprobs: logits must be float32 or bfloat16, got {logits.dtype}")
-    _need(logits.dim() >= 1 and targets.dtype == torch.int64 and targets.shape == logits.shape[:-1],
-          f"token_logprobs: targets must be int64 {tuple(logits.shape[:-1])}, got {tuple(targets.shape)} {targets.dtype}")
+    name = "token_logprobs"
+    if logits.dtype not in _DT:
+        _refuse(name, f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.dim() < 1 or targets.dtype != _I64 or targets.shape != logits.shape[:-1] or targets.device != logits.device:
+        _refuse(name, f"targets must be int64 {tuple(logits.shape[:-1])} on the logits' device, got {_desc(targets)}")
     top, V, shape = int(top), logits.shape[-1], targets.shape
-    _need(V > 0 and 0 <= top <= min(V, MAX_TOP_LOGPROBS), f"token_logprobs: top must lie between 0 and min(V, {MAX_TOP_LOGPROBS}), got {top} (V = {V})")
-    _need(V < 1 << 30 and targets.numel() < 1 << 31, "token_logprobs: fewer than 2^30 columns and 2^31 rows are supported")
-    _need_same_device("token_logprobs", logits, targets)
+    if V < 1 or not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
+        _refuse(name, f"top must lie between 0 and min(V, {MAX_TOP_LOGPROBS}), got {top} (V = {V})")
+    if V >= 1 << 30 or targets.numel() >= 1 << 31:
+        _refuse(name, "fewer than 2^30 columns and 2^31 rows are supported")
     x = logits if logits.dim() == 3 else logits[None] if logits.dim() == 2 else logits.reshape(1, -1, V)
     if V > 1 and x.stride(2) != 1:
         x = x.contiguous()
