@@ -1,16 +1,19 @@
 // token_logprobs.hip -- log probabilities of given tokens with the entropy of their distribution and its best alternatives, and the gradient of all
 // three with respect to the logits.  Per row x of V logits, target t:
-//   z = log sum exp(x)      logp = x_t - z      H = z - sum_c p_c x_c  (p = exp(x - z); p_c = 0 adds nothing, also where x_c = -inf)
+//   z = log sum exp(x)      logp = x_t - z      H = log s - (sum_c e_c d_c) / s   with d_c = x_c - m, e_c = exp(d_c), s = sum e_c, m = max x
 //   top: the n largest logits, largest first, equal ones by ascending column (a NaN counts as the largest, as torch.topk has it), as x_c - z
-// A target < 0 is no token (logp 0, no gradient from it); a target >= V makes its logp NaN.  A row without a finite logit (all -inf) has
-// z = -inf: logp -inf, entropy 0, alternatives -inf, gradient 0.
+// A target < 0 is no token (logp 0, no gradient from it); a target >= V makes its logp NaN.  A row without a logit above -inf has
+// logp -inf, entropy 0, alternatives -inf, gradient 0.
+//
+// Forward: ONE pass over the row with a running maximum per thread (sums rescaled when it grows: sum e d becomes f (sum e d + delta sum e) with
+// delta = m_old - m_new, f = exp(delta)), 4 x 16 B per thread in flight; m and log s leave the kernel apart, because m + log s in one float loses
+// log s where the logits sit far from 0.  Backward: one streaming pass, p recomputed from them.
+// Alternatives: the n-th largest of a wave's 64 per-thread maxima is a lower bound of the row's n-th largest logit (n logits >= it exist); the largest
+// such bound L of the waves leaves a few dozen candidates, and only the threads whose own maximum reaches L look at their logits again.  The
+// candidates are ranked by (value, column) in LDS, so the order in which they were collected does not matter.  Rows where that fails (fewer than n logits
+// above the bound: -inf columns; thousands of equal logits; NaN) take n exact passes instead.
 #include "common.h"
-
-template <typename T> __device__ __forceinline__ float lp_ld(const T* p);
-template <> __device__ __forceinline__ float lp_ld<float>(const float* p) { return *p; }
-template <> __device__ __forceinline__ float lp_ld<bf16_t>(const bf16_t* p) { return bf16_to_f32(*p); }
-__device__ __forceinline__ void lp_st(float* p, float v) { *p = v; }
-__device__ __forceinline__ void lp_st(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+#include <float.h>
 
 // ascending unsigned order of the values; -0 and +0 are one value, every NaN the largest
 __device__ __forceinline__ uint32_t lp_key(float x) {
@@ -18,99 +21,250 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+#define LP_LOG2E 1.4426950408889634f
+#define LP_FLOOR -200.f          // exp of anything below is 0: d is cut here where it meets a factor of 0 (0 * -inf would be NaN)
+#define LP_CAND 512
+#define LP_U 4                   // 16-byte pieces per thread in flight
+
+// 16 bytes of a row, whatever its alignment (rows of an odd width start anywhere; the loads stay 16 bytes wide)
+typedef uint32_t lp_u4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t lp_u4a4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct LpVec;
+template <> struct LpVec<bf16_t> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ float at(const bf16_t* p) { return bf16_to_f32(*p); }
+    static __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+    static __device__ __forceinline__ uint4 load(const bf16_t* p) { return __builtin_bit_cast(uint4, *reinterpret_cast<const lp_u4a2*>(p)); }
+    static __device__ __forceinline__ void unpack(const uint4 v, float* f) { unpack8(v, f); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *reinterpret_cast<lp_u4a2*>(p) = __builtin_bit_cast(lp_u4a2, pack8(f)); }
+};
+template <> struct LpVec<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ float at(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ uint4 load(const float* p) { return __builtin_bit_cast(uint4, *reinterpret_cast<const lp_u4a4*>(p)); }
+    static __device__ __forceinline__ void unpack(const uint4 v, float* f) {
+        f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<lp_u4a4*>(p) = lp_u4a4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}; }
+};
 
 struct LogprobArgs {
     const void* x; int64_t ld_outer, ld_inner; int inner;      // row r starts at (r / inner) * ld_outer + (r % inner) * ld_inner
     const int64_t* target; int V, top; float* logp; float* ent; float* stats; float* top_logp; int64_t* top_ids;
 };
 
-#define LP_THREADS 256
-__device__ __forceinline__ float lp_block(float v, float* sh, bool is_max) {
-    v = is_max ? wave_max(v) : wave_sum(v);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = sh[0];
-    for (int i = 1; i < LP_THREADS / 64; ++i) r = is_max ? fmaxf(r, sh[i]) : r + sh[i];
-    __syncthreads();
-    return r;
-}
-
-template <typename T>
-__global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LogprobArgs p) {
-    __shared__ float sh[LP_THREADS / 64];
-    __shared__ uint64_t best[LP_THREADS / 64];
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
-    float m = -INFINITY;
-    for (int c = tid; c < p.V; c += LP_THREADS) m = fmaxf(m, lp_ld(x + c));
-    m = lp_block(m, sh, true);
-    const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f, w = 0.f;
-    for (int c = tid; c < p.V; c += LP_THREADS) {
-        const float d = lp_ld(x + c) - base, e = expf(d);
-        s += e;
-        if (e != 0.f) w = fmaf(e, d, w);
+// running (maximum, sum e, sum e d) of a thread
+struct LpSum {
+    float m = -FLT_MAX, s = 0.f, w = 0.f;                      // (not -inf: -inf - -inf; a logit of -FLT_MAX itself still counts)
+    __device__ __forceinline__ void rise(float to) {
+        const float d = m - to, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        w = f * fmaf(fmaxf(d, LP_FLOOR), s, w);
+        s *= f;
+        m = to;
     }
-    s = lp_block(s, sh, false);
-    w = lp_block(w, sh, false);
+    __device__ __forceinline__ void add(float x) {
+        const float d = x - m, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        s += e;
+        w = fmaf(e, fmaxf(d, LP_FLOOR), w);
+    }
+};
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobArgs p) {
+    using Vec = LpVec<T>;
+    constexpr int E = Vec::E, WAVES = THREADS / 64;
+    __shared__ float sh[3][WAVES];
+    __shared__ float s_bound[WAVES];
+    __shared__ uint64_t s_best[WAVES];
+    __shared__ float c_val[LP_CAND];
+    __shared__ int c_idx[LP_CAND];
+    __shared__ int s_n;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
+    const int full = p.V / E;                                   // whole pieces; the rest is read element by element
+    if (tid == 0) s_n = 0;
+    LpSum a;
+    int ch = tid;
+    for (; ch + (LP_U - 1) * THREADS < full; ch += LP_U * THREADS) {
+        uint4 raw[LP_U];
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+        float f[LP_U][E], mx = -FLT_MAX;
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            Vec::unpack(raw[u], f[u]);
+#pragma unroll
+            for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[u][j]);
+        }
+        if (mx > a.m) a.rise(mx);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+            for (int j = 0; j < E; ++j) a.add(f[u][j]);
+    }
+    for (; ch < full; ch += THREADS) {
+        float f[E], mx = -FLT_MAX;
+        Vec::unpack(Vec::load(x + (int64_t)ch * E), f);
+#pragma unroll
+        for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
+        if (mx > a.m) a.rise(mx);
+#pragma unroll
+        for (int j = 0; j < E; ++j) a.add(f[j]);
+    }
+    const int rest = full * E + tid;                            // the last V % E logits, one thread each
+    if (rest < p.V) {
+        const float v = Vec::at(x + rest);
+        if (v > a.m) a.rise(v);
+        a.add(v);
+    }
+    const float mine = a.m;                                     // this thread's own maximum
+    // the row's sums
+    float m = wave_max(a.m);
+    if (lane == 0) sh[0][wave] = m;
+    __syncthreads();
+    m = sh[0][0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) m = fmaxf(m, sh[0][i]);
+    a.rise(m);
+    const float ws = wave_sum(a.s), ww = wave_sum(a.w);
+    if (lane == 0) { sh[1][wave] = ws; sh[2][wave] = ww; }
+    // (the alternatives' bound in the same round: n times the wave's largest remaining maximum)
+    if (p.top > 0) {
+        float cur = mine, bound = -FLT_MAX;
+        for (int k = 0; k < p.top; ++k) {
+            bound = wave_max(cur);
+            if (cur == bound) cur = -FLT_MAX;
+        }
+        if (lane == 0) s_bound[wave] = bound;
+    }
+    __syncthreads();
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) { s += sh[1][i]; w += sh[2][i]; }
     const float ls = logf(s);
     if (tid == 0) {
         const int64_t t = p.target[r];
-        p.stats[2 * (int64_t)r] = base;                          // z in two parts: base + ls would round away log s where the logits are far from 0
+        p.stats[2 * (int64_t)r] = m;
         p.stats[2 * (int64_t)r + 1] = ls;
         p.ent[r] = s == 0.f ? 0.f : ls - w / s;
-        p.logp[r] = t < 0 ? 0.f : (t >= p.V ? NAN : (s == 0.f ? -INFINITY : (lp_ld(x + t) - base) - ls));
+        p.logp[r] = t < 0 ? 0.f : (t >= p.V ? NAN : (s == 0.f ? -INFINITY : (Vec::at(x + t) - m) - ls));
+    }
+    if (p.top == 0) return;
+    float L = s_bound[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) L = fmaxf(L, s_bound[i]);
+    if (mine >= L) {
+        auto look = [&](int c, float v) {
+            if (v >= L) {
+                const int at = atomicAdd(&s_n, 1);
+                if (at < LP_CAND) { c_val[at] = v; c_idx[at] = c; }
+            }
+        };
+        for (int c = tid; c < full; c += THREADS) {
+            float f[E];
+            Vec::unpack(Vec::load(x + (int64_t)c * E), f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) look(c * E + j, f[j]);
+        }
+        if (rest < p.V) look(rest, Vec::at(x + rest));
+    }
+    __syncthreads();
+    const int n = s_n;
+    float* out = p.top_logp + (int64_t)r * p.top;
+    int64_t* ids = p.top_ids + (int64_t)r * p.top;
+    if (n >= p.top && n <= LP_CAND && s == s) {
+        for (int i = tid; i < n; i += THREADS) {
+            const float v = c_val[i]; const int c = c_idx[i];
+            int above = 0;
+            for (int j = 0; j < n; ++j) { const float o = c_val[j]; above += (o > v || (o == v && c_idx[j] < c)) ? 1 : 0; }
+            if (above < p.top) { ids[above] = c; out[above] = (v - m) - ls; }
+        }
+        return;
     }
     uint64_t last = ~0ull;                                      // (value key, V - 1 - column): descending order of it is the wanted order
     for (int k = 0; k < p.top; ++k) {
         uint64_t b = 0;
-        for (int c = tid; c < p.V; c += LP_THREADS) {
-            const uint64_t key = ((uint64_t)lp_key(lp_ld(x + c)) << 32) | (uint32_t)(p.V - 1 - c);
+        for (int c = tid; c < p.V; c += THREADS) {
+            const uint64_t key = ((uint64_t)lp_key(Vec::at(x + c)) << 32) | (uint32_t)(p.V - 1 - c);
             if (key < last && key > b) b = key;
         }
+#pragma unroll
         for (int d = 32; d; d >>= 1) {
             const uint32_t lo = __shfl_xor((int)(uint32_t)b, d), hi = __shfl_xor((int)(b >> 32), d);
             const uint64_t o = ((uint64_t)hi << 32) | lo;
             b = o > b ? o : b;
         }
-        if ((tid & 63) == 0) best[tid >> 6] = b;
+        if (lane == 0) s_best[wave] = b;
         __syncthreads();
-        for (int i = 0; i < LP_THREADS / 64; ++i) b = best[i] > b ? best[i] : b;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) b = s_best[i] > b ? s_best[i] : b;
         __syncthreads();
         last = b;
         if (tid == 0) {
             const int c = p.V - 1 - (int)(uint32_t)b;
-            p.top_ids[(int64_t)r * p.top + k] = c;
-            p.top_logp[(int64_t)r * p.top + k] = s == 0.f ? -INFINITY : (lp_ld(x + c) - base) - ls;
+            ids[k] = c;
+            out[k] = s == 0.f ? -INFINITY : (Vec::at(x + c) - m) - ls;
         }
     }
 }
 
-// dx_c = -(g_l + sum_k g_k) p_c - g_h p_c (log p_c + H)  + g_l [c = t] + sum_k g_k [c = id_k]
+// dx_c = -p_c (g_l + sum_k g_k + g_h (log p_c + H))  + g_l [c = t] + sum_k g_k [c = id_k]
 struct LogprobGradArgs {
     const void* x; int64_t ld_outer, ld_inner; int inner; const int64_t* target; int V, top; const float* stats; const float* ent; const int64_t* top_ids;
     const float* g_logp; const float* g_ent; const float* g_top; void* dx; int64_t ld_dx;
 };
-template <typename T>
-__global__ __launch_bounds__(LP_THREADS) void token_logprobs_bwd_kernel(const LogprobGradArgs p) {
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const LogprobGradArgs p) {
+    using Vec = LpVec<T>;
+    constexpr int E = Vec::E;
     const int r = blockIdx.x, tid = threadIdx.x;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
     T* dx = (T*)p.dx + r * p.ld_dx;
     const int64_t t = p.target[r];
-    const float base = p.stats[2 * (int64_t)r], ls = p.stats[2 * (int64_t)r + 1], H = p.ent[r];
-    if (ls == -INFINITY) {                                       // nothing in the row: its outputs are constants
-        for (int c = tid; c < p.V; c += LP_THREADS) lp_st(dx + c, 0.f);
-        return;
+    const float m = p.stats[2 * (int64_t)r], ls = p.stats[2 * (int64_t)r + 1], H = p.ent[r];
+    const int full = p.V / E, rest = full * E + tid;
+    const bool empty = ls == -INFINITY;                         // nothing in the row: its outputs are constants
+    const float gl = !p.g_logp || t < 0 || empty ? 0.f : (t < p.V ? p.g_logp[r] : NAN), gh = p.g_ent && !empty ? p.g_ent[r] : 0.f;
+    const int top = p.g_top && !empty ? p.top : 0;
+    float g0 = gl;
+    for (int k = 0; k < top; ++k) g0 += p.g_top[(int64_t)r * p.top + k];
+    g0 = fmaf(gh, H, g0);
+    auto grad = [&](float v) {                                  // without the single columns' own terms
+        const float lp = (v - m) - ls, e = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
+        return empty ? 0.f : -e * fmaf(gh, fmaxf(lp, LP_FLOOR), g0);
+    };
+    int ch = tid;
+    for (; ch + (LP_U - 1) * THREADS < full; ch += LP_U * THREADS) {
+        uint4 raw[LP_U];
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            float f[E];
+            Vec::unpack(raw[u], f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) f[j] = grad(f[j]);
+            Vec::store(dx + (int64_t)(ch + u * THREADS) * E, f);
+        }
     }
-    const float gl = p.g_logp && t >= 0 ? (t < p.V ? p.g_logp[r] : NAN) : 0.f, gh = p.g_ent ? p.g_ent[r] : 0.f;
-    float gt = gl;
-    for (int k = 0; k < p.top; ++k) gt += p.g_top ? p.g_top[(int64_t)r * p.top + k] : 0.f;
-    for (int c = tid; c < p.V; c += LP_THREADS) {
-        const float lp = (lp_ld(x + c) - base) - ls, e = expf(lp);
-        float d = e == 0.f ? 0.f : -e * (gt + gh * (lp + H));
-        if (c == t) d += gl;
-        if (p.g_top) for (int k = 0; k < p.top; ++k) if (p.top_ids[(int64_t)r * p.top + k] == c) d += p.g_top[(int64_t)r * p.top + k];
-        lp_st(dx + c, d);
+    for (; ch < full; ch += THREADS) {
+        float f[E];
+        Vec::unpack(Vec::load(x + (int64_t)ch * E), f);
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = grad(f[j]);
+        Vec::store(dx + (int64_t)ch * E, f);
+    }
+    if (rest < p.V) Vec::put(dx + rest, grad(Vec::at(x + rest)));
+    // the target's and the alternatives' columns once more, with their own terms (whole values, not added to the rounded ones)
+    __syncthreads();
+    if (tid <= top) {
+        const int64_t c = tid < top ? p.top_ids[(int64_t)r * p.top + tid] : t;
+        if (c >= 0 && c < p.V) {
+            float d = grad(Vec::at(x + c)) + (c == t ? gl : 0.f);
+            for (int k = 0; k < top; ++k) d += p.top_ids[(int64_t)r * p.top + k] == c ? p.g_top[(int64_t)r * p.top + k] : 0.f;
+            Vec::put(dx + c, d);
+        }
     }
 }
 
@@ -120,6 +274,18 @@ static int logprob_check(const void* x, int R, int inner, int V, int top, int dt
     VM_REQUIRE(dtype == VM_F32 || dtype == VM_BF16, "%s: dtype must be VM_F32 or VM_BF16", what);
     return VM_OK;
 }
+// 1024 threads a row while the rows alone would leave the chip's 256 CUs short of threads, 256 otherwise
+#define LP_LAUNCH(KERNEL, R, ARGS)                                                                                                       \
+    do {                                                                                                                                 \
+        if (R <= 512) {                                                                                                                  \
+            if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, 1024>), dim3(R), dim3(1024), 0, s, ARGS);                             \
+            else hipLaunchKernelGGL((KERNEL<bf16_t, 1024>), dim3(R), dim3(1024), 0, s, ARGS);                                            \
+        } else {                                                                                                                         \
+            if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, 256>), dim3(R), dim3(256), 0, s, ARGS);                               \
+            else hipLaunchKernelGGL((KERNEL<bf16_t, 256>), dim3(R), dim3(256), 0, s, ARGS);                                              \
+        }                                                                                                                                \
+    } while (0)
+
 extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
                                      float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids, int dtype, void* stream) {
     if (int rc = logprob_check(logits, R, inner, V, top, dtype, "vm_token_logprobs_fwd")) return rc;
@@ -127,8 +293,7 @@ extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64
     LogprobArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, logp, entropy, stats, top_logp, top_ids};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 4.0 : 2.0) * R * (double)V, s, "token_logprobs_r%d_V%d_k%d", R, V, top);
-    if (dtype == VM_F32) hipLaunchKernelGGL(token_logprobs_kernel<float>, dim3(R), dim3(LP_THREADS), 0, s, a);
-    else hipLaunchKernelGGL(token_logprobs_kernel<bf16_t>, dim3(R), dim3(LP_THREADS), 0, s, a);
+    LP_LAUNCH(token_logprobs_kernel, R, a);
     return vm_check_launch("vm_token_logprobs_fwd");
 }
 extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
@@ -139,7 +304,6 @@ extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64
     LogprobGradArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, stats, entropy, top_ids, g_logp, g_entropy, top ? g_top : nullptr, dlogits, ld_dlogits};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 8.0 : 4.0) * R * (double)V, s, "token_logprobs_bwd_r%d_V%d_k%d", R, V, top);
-    if (dtype == VM_F32) hipLaunchKernelGGL(token_logprobs_bwd_kernel<float>, dim3(R), dim3(LP_THREADS), 0, s, a);
-    else hipLaunchKernelGGL(token_logprobs_bwd_kernel<bf16_t>, dim3(R), dim3(LP_THREADS), 0, s, a);
+    LP_LAUNCH(token_logprobs_bwd_kernel, R, a);
     return vm_check_launch("vm_token_logprobs_bwd");
 }
