@@ -9,7 +9,8 @@
 // delta = m_old - m_new, f = exp(delta)), 4 x 16 B per thread in flight; m and log s leave the kernel apart, because m + log s in one float loses
 // log s where the logits sit far from 0.  Backward: one streaming pass, p recomputed from them.
 // Alternatives: the n-th largest of a wave's 64 per-thread maxima is a lower bound of the row's n-th largest logit (n logits >= it exist); the largest
-// such bound L of the waves leaves a few dozen candidates, and only the threads whose own maximum reaches L look at their logits again.  The
+// such bound L of the waves leaves a few dozen candidates, all of them with the threads whose own maximum reaches L: only those threads' pieces are
+// read again (from the caches), dealt out to the whole workgroup.  The
 // candidates are ranked by (value, column) in LDS, so the order in which they were collected does not matter.  Rows where that fails (fewer than n logits
 // above the bound: -inf columns; thousands of equal logits; NaN) take n exact passes instead.
 #include "common.h"
@@ -24,7 +25,7 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
 #define LP_LOG2E 1.4426950408889634f
 #define LP_FLOOR -200.f          // exp of anything below is 0: d is cut here where it meets a factor of 0 (0 * -inf would be NaN)
 #define LP_CAND 512
-#define LP_U 4                   // 16-byte pieces per thread in flight
+#define LP_U 4                   // 16-byte pieces per thread in flight (2, 3 and 8 measured the same within 3 %, 16 a third slower: fewer waves)
 
 // 16 bytes of a row, whatever its alignment (rows of an odd width start anywhere; the loads stay 16 bytes wide)
 typedef uint32_t lp_u4a2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -36,8 +37,12 @@ template <> struct LpVec<bf16_t> {
     static __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
     static __device__ __forceinline__ uint4 load(const bf16_t* p) { return __builtin_bit_cast(uint4, *reinterpret_cast<const lp_u4a2*>(p)); }
     static __device__ __forceinline__ void unpack(const uint4 v, float* f) { unpack8(v, f); }
-    static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *reinterpret_cast<lp_u4a2*>(p) = __builtin_bit_cast(lp_u4a2, pack8(f)); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float* f) { __builtin_nontemporal_store(__builtin_bit_cast(lp_u4a2, pack8(f)), reinterpret_cast<lp_u4a2*>(p)); }
 };
+// (what a thread without a piece works on: logits of -inf, which change no sum)
+template <typename T> __device__ __forceinline__ uint4 lp_none();
+template <> __device__ __forceinline__ uint4 lp_none<bf16_t>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+template <> __device__ __forceinline__ uint4 lp_none<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 template <> struct LpVec<float> {
     static constexpr int E = 4;
     static __device__ __forceinline__ float at(const float* p) { return *p; }
@@ -46,7 +51,7 @@ template <> struct LpVec<float> {
     static __device__ __forceinline__ void unpack(const uint4 v, float* f) {
         f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
     }
-    static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<lp_u4a4*>(p) = lp_u4a4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}; }
+    static __device__ __forceinline__ void store(float* p, const float* f) { __builtin_nontemporal_store(lp_u4a4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}, reinterpret_cast<lp_u4a4*>(p)); }
 };
 
 struct LogprobArgs {
@@ -79,17 +84,20 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     __shared__ uint64_t s_best[WAVES];
     __shared__ float c_val[LP_CAND];
     __shared__ int c_idx[LP_CAND];
-    __shared__ int s_n;
+    __shared__ int s_list[THREADS];
+    __shared__ int s_n, s_owners;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
     const int full = p.V / E;                                   // whole pieces; the rest is read element by element
-    if (tid == 0) s_n = 0;
+    if (tid == 0) s_n = s_owners = 0;
     LpSum a;
-    int ch = tid;
-    for (; ch + (LP_U - 1) * THREADS < full; ch += LP_U * THREADS) {
+    for (int ch = tid; ch < full; ch += LP_U * THREADS) {
         uint4 raw[LP_U];
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+        for (int u = 0; u < LP_U; ++u) {
+            raw[u] = lp_none<T>();
+            if (ch + u * THREADS < full) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+        }
         float f[LP_U][E], mx = -FLT_MAX;
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
@@ -102,15 +110,6 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         for (int u = 0; u < LP_U; ++u)
 #pragma unroll
             for (int j = 0; j < E; ++j) a.add(f[u][j]);
-    }
-    for (; ch < full; ch += THREADS) {
-        float f[E], mx = -FLT_MAX;
-        Vec::unpack(Vec::load(x + (int64_t)ch * E), f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
-        if (mx > a.m) a.rise(mx);
-#pragma unroll
-        for (int j = 0; j < E; ++j) a.add(f[j]);
     }
     const int rest = full * E + tid;                            // the last V % E logits, one thread each
     if (rest < p.V) {
@@ -145,8 +144,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     const float ls = logf(s);
     if (tid == 0) {
         const int64_t t = p.target[r];
-        p.stats[2 * (int64_t)r] = m;
-        p.stats[2 * (int64_t)r + 1] = ls;
+        if (p.stats) { p.stats[2 * (int64_t)r] = m; p.stats[2 * (int64_t)r + 1] = ls; }
         p.ent[r] = s == 0.f ? 0.f : ls - w / s;
         p.logp[r] = t < 0 ? 0.f : (t >= p.V ? NAN : (s == 0.f ? -INFINITY : (Vec::at(x + t) - m) - ls));
     }
@@ -154,20 +152,29 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     float L = s_bound[0];
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) L = fmaxf(L, s_bound[i]);
-    if (mine >= L) {
-        auto look = [&](int c, float v) {
-            if (v >= L) {
-                const int at = atomicAdd(&s_n, 1);
-                if (at < LP_CAND) { c_val[at] = v; c_idx[at] = c; }
-            }
-        };
-        for (int c = tid; c < full; c += THREADS) {
-            float f[E];
-            Vec::unpack(Vec::load(x + (int64_t)c * E), f);
-#pragma unroll
-            for (int j = 0; j < E; ++j) look(c * E + j, f[j]);
+    auto look = [&](int c, float v) {
+        if (v >= L) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < LP_CAND) { c_val[at] = v; c_idx[at] = c; }
         }
-        if (rest < p.V) look(rest, Vec::at(x + rest));
+    };
+    if (mine >= L) s_list[atomicAdd(&s_owners, 1)] = tid;
+    if (rest < p.V) look(rest, Vec::at(x + rest));
+    __syncthreads();
+    // the owners' pieces once more, dealt out to all threads
+    const int owners = s_owners, pieces = owners * ((full + THREADS - 1) / THREADS);
+    for (int i = tid; i < pieces; i += THREADS) {
+        const int turn = i / owners, ch = s_list[i - turn * owners] + turn * THREADS;
+        if (ch < full) {
+            float f[E], mx = -INFINITY;
+            Vec::unpack(Vec::load(x + (int64_t)ch * E), f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
+            if (mx >= L) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) look(ch * E + j, f[j]);
+            }
+        }
     }
     __syncthreads();
     const int n = s_n;
@@ -218,7 +225,7 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const LogprobGradArgs p) {
     using Vec = LpVec<T>;
     constexpr int E = Vec::E;
-    const int r = blockIdx.x, tid = threadIdx.x;
+    const int r = gridDim.x - 1 - blockIdx.x, tid = threadIdx.x;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
     T* dx = (T*)p.dx + r * p.ld_dx;
     const int64_t t = p.target[r];
@@ -234,26 +241,22 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const Logpr
         const float lp = (v - m) - ls, e = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
         return empty ? 0.f : -e * fmaf(gh, fmaxf(lp, LP_FLOOR), g0);
     };
-    int ch = tid;
-    for (; ch + (LP_U - 1) * THREADS < full; ch += LP_U * THREADS) {
+    for (int ch = tid; ch < full; ch += LP_U * THREADS) {
         uint4 raw[LP_U];
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+        for (int u = 0; u < LP_U; ++u) {
+            raw[u] = lp_none<T>();
+            if (ch + u * THREADS < full) raw[u] = Vec::load(x + (int64_t)(ch + u * THREADS) * E);
+        }
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
+            if (ch + u * THREADS >= full) break;
             float f[E];
             Vec::unpack(raw[u], f);
 #pragma unroll
             for (int j = 0; j < E; ++j) f[j] = grad(f[j]);
             Vec::store(dx + (int64_t)(ch + u * THREADS) * E, f);
         }
-    }
-    for (; ch < full; ch += THREADS) {
-        float f[E];
-        Vec::unpack(Vec::load(x + (int64_t)ch * E), f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) f[j] = grad(f[j]);
-        Vec::store(dx + (int64_t)ch * E, f);
     }
     if (rest < p.V) Vec::put(dx + rest, grad(Vec::at(x + rest)));
     // the target's and the alternatives' columns once more, with their own terms (whole values, not added to the rounded ones)
@@ -275,25 +278,24 @@ static int logprob_check(const void* x, int R, int inner, int V, int top, int dt
     return VM_OK;
 }
 // 1024 threads a row while the rows alone would leave the chip's 256 CUs short of threads, 256 otherwise
-#define LP_LAUNCH(KERNEL, R, ARGS)                                                                                                       \
-    do {                                                                                                                                 \
-        if (R <= 512) {                                                                                                                  \
-            if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, 1024>), dim3(R), dim3(1024), 0, s, ARGS);                             \
-            else hipLaunchKernelGGL((KERNEL<bf16_t, 1024>), dim3(R), dim3(1024), 0, s, ARGS);                                            \
-        } else {                                                                                                                         \
-            if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, 256>), dim3(R), dim3(256), 0, s, ARGS);                               \
-            else hipLaunchKernelGGL((KERNEL<bf16_t, 256>), dim3(R), dim3(256), 0, s, ARGS);                                              \
-        }                                                                                                                                \
+#ifndef LP_WIDE_ROWS
+#define LP_WIDE_ROWS 2048
+#endif
+#define LP_LAUNCH(KERNEL, T)                                                                          \
+    do {                                                                                              \
+        if (R <= LP_WIDE_ROWS) hipLaunchKernelGGL((KERNEL<T, 1024>), dim3(R), dim3(1024), 0, s, a);   \
+        else hipLaunchKernelGGL((KERNEL<T, 256>), dim3(R), dim3(256), 0, s, a);                       \
     } while (0)
 
 extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
                                      float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids, int dtype, void* stream) {
     if (int rc = logprob_check(logits, R, inner, V, top, dtype, "vm_token_logprobs_fwd")) return rc;
-    VM_REQUIRE(targets && logp && entropy && stats && (top == 0 || (top_logp && top_ids)), "vm_token_logprobs_fwd: null pointer");
+    VM_REQUIRE(targets && logp && entropy && (top == 0 || (top_logp && top_ids)), "vm_token_logprobs_fwd: null pointer");
     LogprobArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, logp, entropy, stats, top_logp, top_ids};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 4.0 : 2.0) * R * (double)V, s, "token_logprobs_r%d_V%d_k%d", R, V, top);
-    LP_LAUNCH(token_logprobs_kernel, R, a);
+    if (dtype == VM_F32) LP_LAUNCH(token_logprobs_kernel, float);
+    else LP_LAUNCH(token_logprobs_kernel, bf16_t);
     return vm_check_launch("vm_token_logprobs_fwd");
 }
 extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
@@ -304,6 +306,7 @@ extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64
     LogprobGradArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, stats, entropy, top_ids, g_logp, g_entropy, top ? g_top : nullptr, dlogits, ld_dlogits};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 8.0 : 4.0) * R * (double)V, s, "token_logprobs_bwd_r%d_V%d_k%d", R, V, top);
-    LP_LAUNCH(token_logprobs_bwd_kernel, R, a);
+    if (dtype == VM_F32) LP_LAUNCH(token_logprobs_bwd_kernel, float);
+    else LP_LAUNCH(token_logprobs_bwd_kernel, bf16_t);
     return vm_check_launch("vm_token_logprobs_bwd");
 }

@@ -1396,34 +1396,40 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor         # [..., top] int64
 
 
-class TokenLogprobsFn(Fn):
-    """logits as a [A, B, V] view with unit column stride (rows A x B in order: a shifted slice of the decoder's logits needs no copy)"""
+def _token_logprobs_fwd(x, rows, targets, top, stats):
+    """``rows`` = (outer stride, inner stride, rows per outer step): where row r of the logits starts (vm_token_logprobs_fwd)"""
+    shape, V = targets.shape, x.shape[-1]
+    logp = torch.empty(shape, dtype=torch.float32, device=x.device)
+    ent = torch.empty(shape, dtype=torch.float32, device=x.device)
+    best = torch.empty(shape + (top,), dtype=torch.float32, device=x.device)
+    ids = torch.empty(shape + (top,), dtype=_I64, device=x.device)
+    check(lib().vm_token_logprobs_fwd(ptr(x), rows[0], rows[1], rows[2], ptr(targets), targets.numel(), V, top, ptr(logp), ptr(ent), ptr(stats), ptr(best),
+                                      ptr(ids), _DT[x.dtype], stream()), "token_logprobs")
+    return logp, ent, best, ids
 
+
+class TokenLogprobsFn(Fn):
     @staticmethod
-    def forward(ctx, x, targets, top, shape):
-        A, B, V = x.shape
-        logp, ent = (torch.empty(shape, dtype=torch.float32, device=x.device) for _ in range(2))
-        stats = torch.empty(A * B, 2, dtype=torch.float32, device=x.device)
-        best = torch.empty(*shape, top, dtype=torch.float32, device=x.device)
-        ids = torch.empty(*shape, top, dtype=torch.int64, device=x.device)
-        check(lib().vm_token_logprobs_fwd(ptr(x), x.stride(0), x.stride(1), B, ptr(targets), A * B, V, top, ptr(logp), ptr(ent), ptr(stats), ptr(best), ptr(ids),
-                                          _DT[x.dtype], stream()), "vm_token_logprobs_fwd")
-        ctx.save_for_backward(x, targets, stats, ent, ids)
-        ctx.mark_non_differentiable(ids)
+    def forward(ctx, x, rows, targets, top):
+        stats = torch.empty(targets.numel(), 2, dtype=torch.float32, device=x.device)
+        out = _token_logprobs_fwd(x, rows, targets, top, stats)
+        ctx.save_for_backward(x, targets, stats, out[1], out[3])
+        ctx.rows = rows
+        ctx.mark_non_differentiable(out[3])
         ctx.set_materialize_grads(False)
-        return logp, ent, best, ids
+        return out
 
     @staticmethod
     def backward(ctx, g_logp, g_ent, g_top, _g_ids):
         x, targets, stats, ent, ids = ctx.saved_tensors
-        A, B, V = x.shape
-        ld = x.stride(1) if V <= x.stride(1) < V + 8 else V           # the logits' own padded rows, where they have such
-        dx = torch.empty(A * B, ld, dtype=x.dtype, device=x.device)
-        g = [t.float().contiguous() if t is not None else None for t in (g_logp, g_ent, g_top if ids.shape[-1] else None)]
+        rows, V, top = ctx.rows, x.shape[-1], ids.shape[-1]
+        ld = rows[1] if V <= rows[1] < V + 8 else V                   # the logits' own padded rows, where they have such
+        dx = torch.empty(x.shape[:-1] + (ld,), dtype=x.dtype, device=x.device)
+        g = [t.float().contiguous() if t is not None else None for t in (g_logp, g_ent, g_top if top else None)]
         with torch.cuda.device(x.device):
-            check(lib().vm_token_logprobs_bwd(ptr(x), x.stride(0), x.stride(1), B, ptr(targets), A * B, V, ids.shape[-1], ptr(stats), ptr(ent), ptr(ids), ptr(g[0]),
-                                              ptr(g[1]), ptr(g[2]), ptr(dx), ld, _DT[x.dtype], stream()), "vm_token_logprobs_bwd")
-        return dx.view(A, B, ld)[..., :V], None, None, None
+            check(lib().vm_token_logprobs_bwd(ptr(x), rows[0], rows[1], rows[2], ptr(targets), targets.numel(), V, top, ptr(stats), ptr(ent), ptr(ids), ptr(g[0]),
+                                              ptr(g[1]), ptr(g[2]), ptr(dx), ld, _DT[x.dtype], stream()), "token_logprobs")
+        return dx[..., :V] if ld != V else dx, None, None, None
 
 
 @_on_device_of
@@ -1443,10 +1449,20 @@ def token_logprobs(logits, targets, top=0):
         _refuse(name, f"top must lie between 0 and min(V, {MAX_TOP_LOGPROBS}), got {top} (V = {V})")
     if V >= 1 << 30 or targets.numel() >= 1 << 31:
         _refuse(name, "fewer than 2^30 columns and 2^31 rows are supported")
-    x = logits if logits.dim() == 3 else logits[None] if logits.dim() == 2 else logits.reshape(1, -1, V)
-    if V > 1 and x.stride(2) != 1:
-        x = x.contiguous()
     if targets.numel() == 0:
         z = logits.float().sum(-1)
         return TokenLogprobs(z, z.clone(), z.new_zeros(*shape, top), targets.new_zeros(*shape, top))
-    return TokenLogprobs(*TokenLogprobsFn.apply(x, targets.contiguous(), top, shape))
+    x = logits
+    if V > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if x.dim() == 2:
+        rows = (0, x.stride(0), x.shape[0])
+    elif x.dim() == 3:
+        rows = (x.stride(0), x.stride(1), x.shape[1])                 # (logits[:, :-1] of the decoder's [B, L, V] is read where it lies)
+    else:
+        x = x.contiguous()
+        rows = (0, V, targets.numel())
+    targets = targets.contiguous()
+    if torch.is_grad_enabled() and x.requires_grad:
+        return TokenLogprobs(*TokenLogprobsFn.apply(x, rows, targets, top))
+    return TokenLogprobs(*_token_logprobs_fwd(x, rows, targets, top, None))
