@@ -116,6 +116,16 @@ def test_many_rows(dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,top", [(37, 32), (700, 5), (4100, 7)])
+def test_many_rows_of_equal_and_missing_logits(dtype, V, top):
+    x = torch.randint(0, 2, (2050, V), generator=torch.Generator().manual_seed(V)).to(dtype)
+    x[::3] = 1.0
+    x[1::7, top:] = -float("inf")
+    x[2::9, 1:] = -float("inf")
+    check(x, torch.zeros(2050, dtype=torch.int64), top)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("V,top", [(50, 32), (3000, 32), (30522, 32), (40000, 17)])
 def test_equal_logits_are_ordered_by_column(dtype, V, top):
     g = torch.Generator().manual_seed(V)

@@ -361,11 +361,17 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
     }
 }
 
+#ifndef PA_KEYS
+#define PA_KEYS 512
+#endif
+#ifndef PA_BLOCKS
+#define PA_BLOCKS 2048
+#endif
 // how many workgroups share a row's keys
 static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
     const int64_t blocks = (int64_t)N * Hkv * ((Hq / Hkv + 15) / 16);
-    const int64_t keys = (int64_t)M * page_size, most = (keys + 511) / 512;
-    int64_t s = (2048 + blocks - 1) / blocks;
+    const int64_t keys = (int64_t)M * page_size, most = (keys + PA_KEYS - 1) / PA_KEYS;
+    int64_t s = (PA_BLOCKS + blocks - 1) / blocks;
     if (s > most) s = most;
     if (s > PA_MAX_SPLITS) s = PA_MAX_SPLITS;
     return (int)(s < 1 ? 1 : s);

@@ -277,14 +277,15 @@ static int logprob_check(const void* x, int R, int inner, int V, int top, int dt
     VM_REQUIRE(dtype == VM_F32 || dtype == VM_BF16, "%s: dtype must be VM_F32 or VM_BF16", what);
     return VM_OK;
 }
-// 1024 threads a row while the rows alone would leave the chip's 256 CUs short of threads, 256 otherwise
-#ifndef LP_WIDE_ROWS
-#define LP_WIDE_ROWS 2048
-#endif
-#define LP_LAUNCH(KERNEL, T)                                                                          \
-    do {                                                                                              \
-        if (R <= LP_WIDE_ROWS) hipLaunchKernelGGL((KERNEL<T, 1024>), dim3(R), dim3(1024), 0, s, a);   \
-        else hipLaunchKernelGGL((KERNEL<T, 256>), dim3(R), dim3(256), 0, s, a);                       \
+// Threads per row, by the 16-byte pieces of a row.  Forward: one wave where a row is short and there are rows enough to fill the chip with waves (no
+// barriers, many rows in flight): 100000 x 1000 bf16 110 us with 64 threads, 195 with 128, 292 with 256; 20000 x 8832 bf16 86 / 102 / 103;
+// longer rows the other way round: 10000 x 8832 fp32 82 / 76 / 71, 8192 x 30522 bf16 - / 123 / 115.  Backward (no reduction): about one batch of
+// LP_U pieces per thread: 100000 x 1000 bf16 106 us with 64 threads, 144 with 128, 176 with 256, 676 with 1024; 20000 x 8832 bf16 111 with 256, 118 with 512, 184
+// with 1024; 10000 x 8832 fp32 116 / 108 / 120; 8192 x 30522 bf16 169 / 164 / 157.
+#define LP_LAUNCH(KERNEL, THREADS)                                                                                          \
+    do {                                                                                                                    \
+        if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, THREADS>), dim3(R), dim3(THREADS), 0, s, a);                 \
+        else hipLaunchKernelGGL((KERNEL<bf16_t, THREADS>), dim3(R), dim3(THREADS), 0, s, a);                                \
     } while (0)
 
 extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
@@ -294,8 +295,8 @@ extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64
     LogprobArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, logp, entropy, stats, top_logp, top_ids};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 4.0 : 2.0) * R * (double)V, s, "token_logprobs_r%d_V%d_k%d", R, V, top);
-    if (dtype == VM_F32) LP_LAUNCH(token_logprobs_kernel, float);
-    else LP_LAUNCH(token_logprobs_kernel, bf16_t);
+    if (V / (dtype == VM_F32 ? 4 : 8) <= 1536 && R >= 2048) LP_LAUNCH(token_logprobs_kernel, 64);
+    else LP_LAUNCH(token_logprobs_kernel, 256);
     return vm_check_launch("vm_token_logprobs_fwd");
 }
 extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
@@ -306,7 +307,10 @@ extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64
     LogprobGradArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, stats, entropy, top_ids, g_logp, g_entropy, top ? g_top : nullptr, dlogits, ld_dlogits};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 8.0 : 4.0) * R * (double)V, s, "token_logprobs_bwd_r%d_V%d_k%d", R, V, top);
-    if (dtype == VM_F32) LP_LAUNCH(token_logprobs_bwd_kernel, float);
-    else LP_LAUNCH(token_logprobs_bwd_kernel, bf16_t);
+    const int want = V / (dtype == VM_F32 ? 4 : 8) / LP_U;
+    if (want <= 96) LP_LAUNCH(token_logprobs_bwd_kernel, 64);
+    else if (want <= 384) LP_LAUNCH(token_logprobs_bwd_kernel, 256);
+    else if (want <= 704) LP_LAUNCH(token_logprobs_bwd_kernel, 512);
+    else LP_LAUNCH(token_logprobs_bwd_kernel, 1024);
     return vm_check_launch("vm_token_logprobs_bwd");
 }
