@@ -23,9 +23,9 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 struct PagedAttnArgs {
     const void* q; int64_t q_row, q_head; const void* k; const void* v; const int32_t* table; int64_t ld_table; const int32_t* lengths; void* o;
-    float* part_o; float* part_ml; int N, Hq, Hk, G, qblocks, dh, P, shift, M, splits; float scale_log2;
+    float* part_o; float* part_ml; int N, Hq, Hk, G, qblocks, dh, P, shift, M, splits, q_wide; float scale_log2;
 };
-#define PA_WAVES 4
+#define PA_WAVES 4             // of a workgroup that shares a row with others
 __device__ __forceinline__ void pa_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void pa_store(bf16_t* p, float v) { *p = f32_to_bf16(v); }
 
@@ -48,10 +48,18 @@ template <typename T, int W> struct PaTile;
 template <int W> struct PaTile<bf16_t, W> {
     static constexpr int SUB = 2, KC = (16 * W + 31) / 32;       // K fragments of 32 columns: 8 per lane
     static constexpr int VD = W / 2;                              // dwords of V per lane and key
-    uint4 q[KC];
+    struct Q { uint4 q[KC]; };
     uint4 k[SUB][KC];
     uint32_t v[SUB][4][VD];
-    __device__ __forceinline__ void load_q(const bf16_t* row, int g, int dh, bool live) {      // any stride and alignment: element loads
+    static __device__ __forceinline__ void load_q(Q& x, const bf16_t* row, int g, int dh, bool live, bool wide) {      // any stride and alignment
+        if (wide) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                x.q[c] = make_uint4(0, 0, 0, 0);
+                if (live && c * 32 + g * 8 < dh) x.q[c] = *reinterpret_cast<const uint4*>(row + c * 32 + g * 8);
+            }
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             uint32_t w[4];
@@ -60,32 +68,26 @@ template <int W> struct PaTile<bf16_t, W> {
                 const int d = c * 32 + g * 8 + 2 * i;
                 w[i] = live && d < dh ? (uint32_t)row[d] | ((uint32_t)row[d + 1] << 16) : 0u;
             }
-            q[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            x.q[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    // base: the subtile's first key row; lane offsets in elements (r = lane % 16, g = lane / 16)
+    // base: the subtile's first key row; r = lane % 16, g = lane / 16.  Columns that the head does not have (dh < 16 W) are read from its last ones
+    // instead, so that no load hangs on a condition: Q is zero there, and such columns of O are not stored.
     __device__ __forceinline__ void load_k(int u, const bf16_t* base, int r, int g, int dh) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            k[u][c] = make_uint4(0, 0, 0, 0);
-            if (c * 32 + g * 8 < dh) k[u][c] = *reinterpret_cast<const uint4*>(base + r * dh + g * 8 + c * 32);
-        }
+        for (int c = 0; c < KC; ++c) k[u][c] = *reinterpret_cast<const uint4*>(base + r * dh + min(c * 32 + g * 8, dh - 8));
     }
     __device__ __forceinline__ void load_v(int u, const bf16_t* base, int r, int g, int dh) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bf16_t* p = base + (g * 4 + i) * dh + r * W;
-#pragma unroll
-            for (int d = 0; d < VD; ++d) v[u][i][d] = 0;
-            if constexpr (VD == 1) { if (r * W < dh) v[u][i][0] = *reinterpret_cast<const uint32_t*>(p); }
-            else if constexpr (VD == 2) { if (r * W < dh) { const uint2 x = *reinterpret_cast<const uint2*>(p); v[u][i][0] = x.x; v[u][i][1] = x.y; } }
+            const bf16_t* p = base + (g * 4 + i) * dh;
+            if constexpr (VD == 1) v[u][i][0] = *reinterpret_cast<const uint32_t*>(p + min(r * W, dh - W));
+            else if constexpr (VD == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p + min(r * W, dh - W)); v[u][i][0] = x.x; v[u][i][1] = x.y; }
             else {
 #pragma unroll
-                for (int d = 0; d < VD; d += 4) {                 // (16 columns a lane: a row may end behind the first eight)
-                    if (r * W + 2 * d < dh) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(p + 2 * d);
-                        v[u][i][d] = x.x; v[u][i][d + 1] = x.y; v[u][i][d + 2] = x.z; v[u][i][d + 3] = x.w;
-                    }
+                for (int d = 0; d < VD; d += 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p + min(r * W + 2 * d, dh - 8));
+                    v[u][i][d] = x.x; v[u][i][d + 1] = x.y; v[u][i][d + 2] = x.z; v[u][i][d + 3] = x.w;
                 }
             }
         }
@@ -94,13 +96,13 @@ template <int W> struct PaTile<bf16_t, W> {
 #pragma unroll
         for (int d = 0; d < VD; ++d) v[u][i][d] = ok ? v[u][i][d] : 0u;
     }
-    __device__ __forceinline__ void scores(float4_t (&s)[SUB]) const {
+    __device__ __forceinline__ void scores(const Q& x, float4_t (&s)[SUB]) const {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < KC; ++c)
-                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[u][c]), __builtin_bit_cast(bf16x8_t, q[c]), s[u], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[u][c]), __builtin_bit_cast(bf16x8_t, x.q[c]), s[u], 0, 0, 0);
         }
     }
     // O^T += V^T P^T.  A probability goes in as two bf16 parts, hi (truncated) + lo: one bf16 would cost 2^-9 of every probability; the second
@@ -138,37 +140,38 @@ template <int W> struct PaTile<bf16_t, W> {
 
 // fp32: exact products on the f32 matrix instruction (4 columns / 4 keys per step; element j of a lane's 16 B feeds step j)
 template <int W> struct PaTile<float, W> {
-    static constexpr int SUB = W <= 4 ? 2 : 1, KC = W;
-    float4_t q[KC];
+    static constexpr int SUB = 1, KC = W;
+    struct Q { float4_t q[KC]; };
     float4_t k[SUB][KC];
     float v[SUB][4][W];
-    __device__ __forceinline__ void load_q(const float* row, int g, int dh, bool live) {
+    static __device__ __forceinline__ void load_q(Q& x, const float* row, int g, int dh, bool live, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                x.q[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+                if (live && c * 16 + g * 4 < dh) x.q[c] = *reinterpret_cast<const float4_t*>(row + c * 16 + g * 4);
+            }
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[c][i] = live && c * 16 + g * 4 + i < dh ? row[c * 16 + g * 4 + i] : 0.f;
+            for (int i = 0; i < 4; ++i) x.q[c][i] = live && c * 16 + g * 4 + i < dh ? row[c * 16 + g * 4 + i] : 0.f;
     }
     __device__ __forceinline__ void load_k(int u, const float* base, int r, int g, int dh) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            k[u][c] = float4_t{0.f, 0.f, 0.f, 0.f};
-            if (c * 16 + g * 4 < dh) k[u][c] = *reinterpret_cast<const float4_t*>(base + r * dh + g * 4 + c * 16);
-        }
+        for (int c = 0; c < KC; ++c) k[u][c] = *reinterpret_cast<const float4_t*>(base + r * dh + min(c * 16 + g * 4, dh - 4));
     }
     __device__ __forceinline__ void load_v(int u, const float* base, int r, int g, int dh) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float* p = base + (g * 4 + i) * dh + r * W;
-#pragma unroll
-            for (int d = 0; d < W; ++d) v[u][i][d] = 0.f;
-            if constexpr (W == 2) { if (r * W < dh) { const float2 x = *reinterpret_cast<const float2*>(p); v[u][i][0] = x.x; v[u][i][1] = x.y; } }
+            const float* p = base + (g * 4 + i) * dh;
+            if constexpr (W == 2) { const float2 x = *reinterpret_cast<const float2*>(p + min(r * W, dh - W)); v[u][i][0] = x.x; v[u][i][1] = x.y; }
             else {
 #pragma unroll
                 for (int d = 0; d < W; d += 4) {
-                    if (r * W + d < dh) {
-                        const float4_t x = *reinterpret_cast<const float4_t*>(p + d);
-                        v[u][i][d] = x[0]; v[u][i][d + 1] = x[1]; v[u][i][d + 2] = x[2]; v[u][i][d + 3] = x[3];
-                    }
+                    const float4_t x = *reinterpret_cast<const float4_t*>(p + min(r * W + d, dh - 4));
+                    v[u][i][d] = x[0]; v[u][i][d + 1] = x[1]; v[u][i][d + 2] = x[2]; v[u][i][d + 3] = x[3];
                 }
             }
         }
@@ -177,14 +180,14 @@ template <int W> struct PaTile<float, W> {
 #pragma unroll
         for (int d = 0; d < W; ++d) v[u][i][d] = ok ? v[u][i][d] : 0.f;
     }
-    __device__ __forceinline__ void scores(float4_t (&s)[SUB]) const {
+    __device__ __forceinline__ void scores(const Q& x, float4_t (&s)[SUB]) const {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             s[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < KC; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u][c][i], q[c][i], s[u], 0, 0, 0);
+                for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[u][c][i], x.q[c][i], s[u], 0, 0, 0);
         }
     }
     __device__ __forceinline__ void accumulate(const float4_t (&p)[SUB], float4_t (&o)[W]) const {
@@ -205,8 +208,8 @@ __device__ __forceinline__ void pa_range(int tiles, int parts, int w, int& t0, i
 }
 template <typename T, int W> __host__ __device__ constexpr int pa_tile_keys() { return 16 * PaTile<T, W>::SUB; }
 
-template <typename T, int W>
-__global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const PagedAttnArgs p) {
+template <typename T, int W, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_kernel(const PagedAttnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float pa_sm[];      // [waves][16][2] (m, l) | [waves][queries][dh] O
     constexpr int SUB = PaTile<T, W>::SUB, TK = 16 * SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -215,57 +218,68 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const Pa
     const int qb = b % p.qblocks; b /= p.qblocks;
     const int kv = b % p.Hk, n = b / p.Hk;
     const int h0 = kv * p.G + qb * 16, nq = min(16, p.G - qb * 16);    // this workgroup's query heads
+    const int32_t* row = p.table + n * p.ld_table;
+    // page numbers of 64 subtiles from subtile ``first`` on, one per lane; a row that has no more of them is fetched at once, along with its
+    // length and the queries (entries behind the length are never used)
     const int cap = p.M << p.shift;
+    // (a number outside the pool becomes -1 here, in the branch that fetches it: the walk below then never waits for a load it did not ask for)
+    int first = cap <= 64 * 16 ? 0 : -64, pages = -1;
+    auto fetch = [&](int limit) {
+        const int key = first * 16 + lane * 16;
+        if (key < limit) { const int page = row[key >> p.shift]; pages = page >= 0 && page < p.P ? page : -1; }
+    };
+    if (first == 0) fetch(cap);
+    using Tile = PaTile<T, W>;
+    typename Tile::Q q;
+    Tile::load_q(q, (const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, p.dh, r < nq, p.q_wide);
     const int len = min(max(p.lengths[n], 0), cap), tiles = (len + TK - 1) / TK;
-    int t0, t1;
-    pa_range(tiles, p.splits * PA_WAVES, split * PA_WAVES, t0, t1);
     const bool only = p.splits == 1;
+    int t0, t1;
+    pa_range(tiles, p.splits * WAVES, split * WAVES, t0, t1);
     if (t0 >= t1 && !only) return;                                    // (workgroup-uniform; the join counts the stretches by the same rule)
-    pa_range(tiles, p.splits * PA_WAVES, split * PA_WAVES + wave, t0, t1);
-    PaTile<T, W> x;
-    x.load_q((const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, p.dh, r < nq);
+    pa_range(tiles, p.splits * WAVES, split * WAVES + wave, t0, t1);
     float m = -INFINITY, l = 0.f;
     float4_t o[W];
 #pragma unroll
     for (int d = 0; d < W; ++d) o[d] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const int32_t* row = p.table + n * p.ld_table;
     const int64_t head = (int64_t)kv << p.shift, page_rows = (int64_t)p.Hk << p.shift;
     const int mask = (1 << p.shift) - 1;
-    int pages = 0;
-    for (int t = t0; t < t1; ++t) {
-        const int ahead = (t - t0) * SUB & 63;                        // page numbers of the next 64 subtiles, one per lane
-        if (ahead == 0) {
-            const int key = t * TK + lane * 16;
-            pages = key < len ? row[key >> p.shift] : -1;
-        }
-        bool good[SUB];
+    auto load = [&](Tile& x, bool (&good)[SUB], int t) {
+        if (t * SUB >= first + 64) { first = t * SUB; pages = -1; fetch(len); }
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            const int page = __builtin_amdgcn_readlane(pages, ahead + u);
-            good[u] = page >= 0 && page < p.P;
-            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + ((t * TK + u * 16) & mask)) * p.dh;
+            const int key = t * TK + u * 16, page = __builtin_amdgcn_readlane(pages, (t * SUB - first + u) & 63);
+            good[u] = key < len && page >= 0;
+            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + (key & mask)) * p.dh;
             x.load_k(u, (const T*)p.k + at, r, g, p.dh);
             x.load_v(u, (const T*)p.v + at, r, g, p.dh);
         }
+    };
+    auto use = [&](Tile& x, const bool (&good)[SUB], int t) {
         bool whole = (t + 1) * TK <= len;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) whole = whole && good[u];
         float4_t s[SUB];
-        x.scores(s);
+        x.scores(q, s);
         float mx = m;
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v = s[u][i] * p.scale_log2;
-                if (!whole) {
+            for (int i = 0; i < 4; ++i) s[u][i] *= p.scale_log2;
+        if (!whole) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
                     const bool ok = good[u] && t * TK + u * 16 + g * 4 + i < len;
-                    v = ok ? v : -INFINITY;
+                    s[u][i] = ok ? s[u][i] : -INFINITY;
                     x.drop_v(u, i, ok);
                 }
-                s[u][i] = v;
-                mx = fmaxf(mx, v);
-            }
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[u][i]);
         mx = pa_col_max(mx);
         const float base = mx == -INFINITY ? 0.f : mx;
         const float f = __builtin_amdgcn_exp2f(m - base);             // 0 the first time (m = -inf)
@@ -280,10 +294,35 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const Pa
 #pragma unroll
             for (int i = 0; i < 4; ++i) { s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - base); l += s[u][i]; }
         x.accumulate(s, o);
+    };
+    if (t0 < t1) {
+        Tile a;
+        bool ga[SUB];
+        int t = t0;
+        if constexpr (W <= 8) {                                  // the next tile is on its way while this one is worked on
+            Tile b;
+            bool gb[SUB];
+            load(a, ga, t);
+            for (; t + 2 < t1; t += 2) {
+                load(b, gb, t + 1);
+                use(a, ga, t);
+                load(a, ga, t + 2);
+                use(b, gb, t + 1);
+            }
+            if (t + 1 < t1) {
+                load(b, gb, t + 1);
+                use(a, ga, t);
+                use(b, gb, t + 1);
+            } else {
+                use(a, ga, t);
+            }
+        } else {
+            for (; t < t1; ++t) { load(a, ga, t); use(a, ga, t); }
+        }
     }
     l = pa_col_sum(l);
     float* ml = pa_sm + wave * 32;
-    float* so = pa_sm + PA_WAVES * 32 + wave * nq * p.dh;
+    float* so = pa_sm + WAVES * 32 + wave * nq * p.dh;
     if (g == 0) { ml[2 * r] = m; ml[2 * r + 1] = l; }
     if (r < nq) {
 #pragma unroll
@@ -295,17 +334,17 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const Pa
             }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nq * p.dh; e += 64 * PA_WAVES) {
+    for (int e = threadIdx.x; e < nq * p.dh; e += 64 * WAVES) {
         const int qi = e / p.dh, c = e - qi * p.dh;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < PA_WAVES; ++w) mm = fmaxf(mm, pa_sm[w * 32 + 2 * qi]);
+        for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, pa_sm[w * 32 + 2 * qi]);
         const float base = mm == -INFINITY ? 0.f : mm;
         float acc = 0.f, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < PA_WAVES; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = __builtin_amdgcn_exp2f(pa_sm[w * 32 + 2 * qi] - base);
-            acc = fmaf(f, pa_sm[PA_WAVES * 32 + (w * nq + qi) * p.dh + c], acc);
+            acc = fmaf(f, pa_sm[WAVES * 32 + (w * nq + qi) * p.dh + c], acc);
             sum = fmaf(f, pa_sm[w * 32 + 2 * qi + 1], sum);
         }
         const int64_t out = (int64_t)n * p.Hq + h0 + qi;
@@ -362,7 +401,7 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
 }
 
 #ifndef PA_KEYS
-#define PA_KEYS 512
+#define PA_KEYS 1024
 #endif
 #ifndef PA_BLOCKS
 #define PA_BLOCKS 2048
@@ -383,12 +422,20 @@ extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, i
     return s == 1 ? 0 : (size_t)N * Hq * s * (dh + 2) * sizeof(float);
 }
 
+template <typename T, int W, int WAVES>
+static void pa_launch_waves(const PagedAttnArgs& a, hipStream_t s) {
+    const int nq = a.G < 16 ? a.G : 16;
+    const size_t lds = sizeof(float) * (WAVES * 32 + (size_t)WAVES * nq * a.dh);
+    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((paged_attention_kernel<T, W, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
+}
+#ifndef PA_ONE
+#define PA_ONE 3000
+#endif
 template <typename T, int W>
 static void pa_launch(const PagedAttnArgs& a, hipStream_t s) {
-    const int nq = a.G < 16 ? a.G : 16;
-    const size_t lds = sizeof(float) * (PA_WAVES * 32 + (size_t)PA_WAVES * nq * a.dh);
-    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL((paged_attention_kernel<T, W>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * PA_WAVES), lds, s, a);
+    if (a.splits == 1 && (int64_t)a.N * a.Hk * a.qblocks >= PA_ONE) return pa_launch_waves<T, W, 1>(a, s);
+    pa_launch_waves<T, W, PA_WAVES>(a, s);
     if (a.splits > 1) hipLaunchKernelGGL(paged_attention_join_kernel<T>, dim3(a.N * a.Hq), dim3(256), 0, s, a, pa_tile_keys<T, W>());
 }
 template <typename T>
@@ -413,9 +460,10 @@ extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q
     VM_REQUIRE((int64_t)N * Hq < (1ll << 31) && (int64_t)N * Hkv * qblocks * splits < (1ll << 31), "vm_paged_attention: too many rows x heads");
     const size_t need = vm_paged_attention_ws(N, Hq, Hkv, dh, M, page_size, dtype);
     VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_attention: 16-byte aligned workspace of %zu bytes required", need);
+    const int e = dtype == VM_F32 ? 4 : 2;
     PagedAttnArgs a = {q, q_row_stride, q_head_stride, k_pages, v_pages, block_table, ld_table, lengths, o, (float*)ws,
                        (float*)ws + (size_t)N * Hq * splits * dh, N, Hq, Hkv, Hq / Hkv, qblocks, dh, P, __builtin_ctz(page_size), M, splits,
-                       scale * 1.4426950408889634f};
+                       (((uintptr_t)q | (uintptr_t)(q_row_stride * e) | (uintptr_t)(q_head_stride * e)) % 16) == 0, scale * 1.4426950408889634f};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_ATTN, 0.0, s, "paged_attn_n%d_h%d_k%d_d%d", N, Hq, Hkv, dh);
     if (dtype == VM_F32) pa_launch_w<float>(a, s);
