@@ -16,8 +16,9 @@
 // The free pages are a ring (first in, first out), not a stack: what is taken (from the head) and what is returned (behind the tail) never
 // share a place while the pool holds P pages in all, so the rows can be served in parallel without a hand-over.
 //
-// Phase A, one workgroup: two scans over the rows (tokens; wanted and returned pages packed into one 64-bit scan).  Phase B, any grid: table
-// rows and ring places by wave, slots by token (binary search of the row in cu_tokens).
+// Phase A, one workgroup: two scans over the rows (tokens; wanted and returned pages).  Phase B: table rows and ring places by wave, slots by token
+// (binary search of the row in the token offsets).  A step of a running batch does both in ONE launch of one workgroup, with everything that B needs
+// in LDS; with more rows or tokens B is a launch of its own over the chip.
 struct PlanRow { int len, ofs, cnt, kind; };       // kind 0 refused / nothing, 1 accepted (cnt pages from ring place head + ofs), 2 released (cnt pages back)
 struct PlanRing { int head, count, returned, pad; };
 struct PlanArgs {
@@ -25,33 +26,47 @@ struct PlanArgs {
     int64_t* slots; int64_t* positions; int max_tokens; int32_t* cu; int32_t* granted; PlanRow* rows; PlanRing* snap;
 };
 #define PLAN_THREADS 1024
+#define PLAN_FUSED_ROWS 1024
+#define PLAN_FUSED_TOKENS 4096
+#define PLAN_FULL ((1u << 30) + 1)                // token sums stop here: past every max_tokens, and two of them fit into 32 bits
 
-__device__ __forceinline__ int64_t shfl_up64(int64_t v, int d) {
-    const int lo = __shfl_up((int)(uint32_t)v, d), hi = __shfl_up((int)(v >> 32), d);
-    return ((int64_t)hi << 32) | (uint32_t)lo;
+// inclusive scan over the wave: rows of 16 lanes first (row_shr 1, 2, 4, 8), then lane 15 of each row into the next (row_bcast15, row_bcast31)
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t plan_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
 }
-// inclusive scan over the workgroup's 1024 threads; total of all threads in `total`
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
+__device__ __forceinline__ uint32_t plan_add(uint32_t a, uint32_t b, bool capped) { const uint32_t s = a + b; return capped ? min(s, PLAN_FULL) : s; }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, bool capped) {
+    v = plan_add(v, plan_dpp<0x111, 0xf>(v), capped);
+    v = plan_add(v, plan_dpp<0x112, 0xf>(v), capped);
+    v = plan_add(v, plan_dpp<0x114, 0xf>(v), capped);
+    v = plan_add(v, plan_dpp<0x118, 0xf>(v), capped);
+    v = plan_add(v, plan_dpp<0x142, 0xa>(v), capped);
+    return plan_add(v, plan_dpp<0x143, 0xc>(v), capped);
+}
+// inclusive scans of one or two values over the workgroup; `before` (the sum of earlier calls) is added and moved on
+template <int THREADS> __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_t& before, bool capped) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int64_t o = shfl_up64(v, d); if (lane >= d) v += o; }
+    v = wave_scan(v, capped);
     if (lane == 63) sh[wave] = v;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
-    for (int w = 0; w < PLAN_THREADS / 64; ++w) { const int64_t x = sh[w]; if (w < wave) before += x; total += x; }
-    __syncthreads();
-    return v + before;
+    uint32_t mine = before, all = before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) { const uint32_t x = sh[w]; if (w < wave) mine = plan_add(mine, x, capped); all = plan_add(all, x, capped); }
+    before = all;
+    return plan_add(mine, v, capped);
 }
 
-__device__ __forceinline__ void plan_scan(const PlanArgs& p) {
-    __shared__ int64_t sh[PLAN_THREADS / 64];
+// FUSED: rows and cu are LDS arrays (cu is written to memory as well)
+template <int THREADS, bool FUSED>
+__device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int* cu, PlanRing* snap) {
+    __shared__ uint32_t sh[3][THREADS / 64];
+    __shared__ int s_taken;
     const int tid = threadIdx.x;
     const int head = p.ring[0], count = p.ring[1];
     const int64_t cap = (int64_t)p.M * p.s;
-    int64_t tok_before = 0;
-    int64_t want_before = 0, back_before = 0, taken_all = 0;
-    for (int base = 0; base < p.N; base += PLAN_THREADS) {
+    uint32_t tok_before = 0, want_before = 0, back_before = 0;
+    if (tid == 0) s_taken = 0;
+    for (int base = 0; base < p.N; base += THREADS) {
         const int i = base + tid;
         int64_t L = 0; int n = 0;
         if (i < p.N) {
@@ -59,50 +74,50 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p) {
             L = L < 0 ? 0 : (L > cap ? cap : L);
         }
         const int64_t t = n > 0 ? n : 0;
-        int64_t tot;
-        const int64_t end = tok_before + block_scan(t, sh, tot);
-        tok_before += tot;
+        __syncthreads();                                                   // (sh is free again, s_taken is set)
+        const uint32_t end = block_scan<THREADS>((uint32_t)min(t, (int64_t)PLAN_FULL), sh[0], tok_before, true);
         const int have = (int)((L + p.s - 1) / p.s);
-        const bool fits = n > 0 && L + t <= cap && end <= p.max_tokens;
+        const bool fits = n > 0 && L + t <= cap && end <= (uint32_t)p.max_tokens;
         const int want = fits ? (int)((L + t + p.s - 1) / p.s) - have : 0;
         const int back = n < 0 ? have : 0;
-        const int64_t both = block_scan(((int64_t)want << 32) | (uint32_t)back, sh, tot);      // (sums below 2^31 each: the host checks N * M)
-        const int64_t upto = want_before + (both >> 32);
-        const int64_t back_upto = back_before + (both & 0xffffffff);
-        want_before += tot >> 32; back_before += tot & 0xffffffff;
-        const bool ok = fits && (want == 0 || upto <= count);
-        block_scan(ok ? want : 0, sh, tot);
-        taken_all += tot;
+        const uint32_t upto = block_scan<THREADS>((uint32_t)want, sh[1], want_before, false);       // (below 2^31: the host checks N * M)
+        const uint32_t back_upto = block_scan<THREADS>((uint32_t)back, sh[2], back_before, false);
+        const bool ok = fits && (want == 0 || (int)upto <= count);
+        const bool last = ok && want > 0;                                  // the accepted rows that need pages are a prefix: the largest upto is their sum
+        if (last) atomicMax(&s_taken, (int)upto);
         if (i < p.N) {
             PlanRow r;
             r.len = (int)L;
             r.kind = n < 0 ? 2 : (ok ? 1 : 0);
             r.cnt = n < 0 ? back : (ok ? want : 0);
-            r.ofs = n < 0 ? (int)(back_upto - back) : (int)(upto - want);
-            p.rows[i] = r;
+            r.ofs = n < 0 ? (int)back_upto - back : (int)upto - want;
+            rows[i] = r;
             p.lengths[i] = n < 0 ? 0 : (int)(L + (ok ? t : 0));
             p.granted[i] = ok ? (int)t : 0;
-            p.cu[i + 1] = (int)(end < p.max_tokens ? end : p.max_tokens);
+            const int e = (int)min(end, (uint32_t)p.max_tokens);
+            cu[i + 1] = e;
+            if constexpr (FUSED) p.cu[i + 1] = e;
         }
     }
+    __syncthreads();
     if (tid == 0) {
-        p.cu[0] = 0;
+        cu[0] = 0;
+        if constexpr (FUSED) p.cu[0] = 0;
         const int64_t room = (int64_t)p.P - count;                        // (a count that lies outside [0, P] is the caller's error; nothing is read or written outside)
-        const int returned = (int)(back_before < room ? back_before : (room > 0 ? room : 0));
+        const int returned = (int)((int64_t)back_before < room ? (int64_t)back_before : (room > 0 ? room : 0));
         PlanRing g = {head, count, returned, 0};
-        *p.snap = g;
-        p.ring[0] = (int)(((int64_t)head + taken_all) % p.P);
-        p.ring[1] = (int)(count - taken_all + returned);
+        *snap = g;
+        p.ring[0] = (int)(((int64_t)head + s_taken) % p.P);
+        p.ring[1] = count - s_taken + returned;
     }
 }
 __device__ __forceinline__ int ring_place(int64_t at, int P) { const int r = (int)(at % P); return r < 0 ? r + P : r; }
 
 // table rows and ring places: wave `wave` of `waves`
-__device__ __forceinline__ void plan_rows(const PlanArgs& p, int wave, int waves) {
-    const PlanRing g = *p.snap;
+__device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows, const PlanRing g, int wave, int waves) {
     const int lane = threadIdx.x & 63;
     for (int i = wave; i < p.N; i += waves) {
-        const PlanRow r = p.rows[i];
+        const PlanRow r = rows[i];
         int32_t* row = p.table + (int64_t)i * p.ld_table;
         if (r.kind == 1) {
             const int have = (r.len + p.s - 1) / p.s;
@@ -116,47 +131,65 @@ __device__ __forceinline__ void plan_rows(const PlanArgs& p, int wave, int waves
     }
 }
 // the slot and position of token `t`
-__device__ __forceinline__ void plan_token(const PlanArgs& p, const PlanRing& g, int t) {
+__device__ __forceinline__ void plan_token(const PlanArgs& p, const PlanRow* rows, const int* cu, const PlanRing g, int t) {
     int64_t slot = -1, pos = 0;
-    if (t < p.cu[p.N]) {
+    if (t < cu[p.N]) {
         int lo = 0, hi = p.N;                                             // the last row whose first token is <= t
-        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (p.cu[mid] <= t) lo = mid; else hi = mid; }
-        const PlanRow r = p.rows[lo];
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (cu[mid] <= t) lo = mid; else hi = mid; }
+        const PlanRow r = rows[lo];
         if (r.kind == 1) {
-            pos = r.len + (t - p.cu[lo]);
-            const int have = (r.len + p.s - 1) / p.s, col = (int)(pos / p.s);
+            const int at = r.len + (t - cu[lo]), have = (r.len + p.s - 1) / p.s, col = at / p.s;
             // a page taken in this call is read from the ring: the row of the table may be under construction
             const int page = col >= have ? p.free_pages[ring_place((int64_t)g.head + r.ofs + (col - have), p.P)] : p.table[(int64_t)lo * p.ld_table + col];
-            if (page >= 0 && page < p.P) slot = (int64_t)page * p.s + (pos - (int64_t)col * p.s);
+            pos = at;
+            if (page >= 0 && page < p.P) slot = (int64_t)page * p.s + (at - col * p.s);
         }
     }
     p.slots[t] = slot;
     p.positions[t] = pos;
 }
 
-__global__ __launch_bounds__(PLAN_THREADS) void paged_plan_scan_kernel(const PlanArgs p) { plan_scan(p); }
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_plan_step_kernel(const PlanArgs p) {
+    __shared__ PlanRow rows[PLAN_FUSED_ROWS];
+    __shared__ int cu[PLAN_FUSED_ROWS + 1];
+    __shared__ PlanRing snap;
+    plan_scan<THREADS, true>(p, rows, cu, &snap);
+    __syncthreads();
+    const PlanRing g = snap;
+    plan_rows(p, rows, g, threadIdx.x >> 6, THREADS / 64);
+    for (int t = threadIdx.x; t < p.max_tokens; t += THREADS) plan_token(p, rows, cu, g, t);
+}
+__global__ __launch_bounds__(PLAN_THREADS) void paged_plan_scan_kernel(const PlanArgs p) { plan_scan<PLAN_THREADS, false>(p, p.rows, p.cu, p.snap); }
 __global__ __launch_bounds__(256) void paged_plan_fill_kernel(const PlanArgs p) {
-    plan_rows(p, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
     const PlanRing g = *p.snap;
-    for (int t = blockIdx.x * 256 + threadIdx.x; t < p.max_tokens; t += gridDim.x * 256) plan_token(p, g, t);
+    plan_rows(p, p.rows, g, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
+    for (int t = blockIdx.x * 256 + threadIdx.x; t < p.max_tokens; t += gridDim.x * 256) plan_token(p, p.rows, p.cu, g, t);
 }
 
-extern "C" size_t vm_paged_plan_ws(int N) { return N > 0 ? (size_t)N * sizeof(PlanRow) + sizeof(PlanRing) : 0; }
+static bool plan_fused(int N, int max_tokens) { return N <= PLAN_FUSED_ROWS && max_tokens <= PLAN_FUSED_TOKENS; }
+extern "C" size_t vm_paged_plan_ws(int N, int max_tokens) { return N <= 0 || plan_fused(N, max_tokens) ? 0 : (size_t)N * sizeof(PlanRow) + sizeof(PlanRing); }
 
 extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int64_t ld_table, int N, int M, int32_t* free_pages,
                              int32_t* ring, int P, int page_size, int64_t* slots, int64_t* positions, int max_tokens, int32_t* cu_tokens,
                              int32_t* granted, void* ws, size_t ws_bytes, void* stream) {
-    VM_REQUIRE(lengths && new_tokens && block_table && free_pages && ring && cu_tokens && granted && ws, "vm_paged_plan: null pointer");
+    VM_REQUIRE(lengths && new_tokens && block_table && free_pages && ring && cu_tokens && granted, "vm_paged_plan: null pointer");
     VM_REQUIRE(N > 0 && M > 0 && P > 0 && page_size > 0 && max_tokens >= 0 && ld_table >= M, "vm_paged_plan: bad shape");
     VM_REQUIRE(max_tokens == 0 || (slots && positions), "vm_paged_plan: slots and positions of max_tokens entries required");
     VM_REQUIRE(max_tokens <= (1 << 30), "vm_paged_plan: max_tokens must be at most 2^30");
     VM_REQUIRE((int64_t)N * M < (1ll << 31) && (int64_t)M * page_size < (1ll << 31), "vm_paged_plan: N * M and M * page_size must stay below 2^31");
-    VM_REQUIRE(((uintptr_t)ws % 16) == 0 && ws_bytes >= vm_paged_plan_ws(N), "vm_paged_plan: 16-byte aligned workspace of vm_paged_plan_ws(N) bytes required");
+    const size_t need = vm_paged_plan_ws(N, max_tokens);
+    VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_plan: 16-byte aligned workspace of %zu bytes required", need);
     PlanRow* rows = reinterpret_cast<PlanRow*>(ws);
     PlanArgs a = {lengths, new_tokens, block_table, ld_table, N, M, free_pages, ring, P, page_size, slots, positions, max_tokens, cu_tokens, granted,
                   rows, reinterpret_cast<PlanRing*>(rows + N)};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_DECODE, 16.0 * N + 16.0 * max_tokens, s, "paged_plan_n%d_t%d", N, max_tokens);
+    if (plan_fused(N, max_tokens)) {
+        if (N <= 256 && max_tokens <= 1024) hipLaunchKernelGGL(paged_plan_step_kernel<256>, dim3(1), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(paged_plan_step_kernel<1024>, dim3(1), dim3(1024), 0, s, a);
+        return vm_check_launch("vm_paged_plan");
+    }
     hipLaunchKernelGGL(paged_plan_scan_kernel, dim3(1), dim3(PLAN_THREADS), 0, s, a);
     int blocks = max_tokens > N * 64 ? (max_tokens + 255) / 256 : (N + 3) / 4;
     if (blocks > 2048) blocks = 2048;

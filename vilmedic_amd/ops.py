@@ -1252,8 +1252,8 @@ def _need_inference(name, *tensors):
 
 
 @functools.lru_cache(maxsize=1024)
-def _plan_ws(N):
-    return lib().vm_paged_plan_ws(N)
+def _plan_ws(N, max_tokens):
+    return lib().vm_paged_plan_ws(N, max_tokens)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1297,17 +1297,16 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
     if N * M >= 1 << 31 or M * page_size >= 1 << 31:
         _refuse(name, "the table's size and M * page_size must stay below 2^31")
     p = [ptr(t) for t in (lengths, new_tokens, block_table, free_pages, free_ring)]
-    # one allocation: slots | positions (8 bytes each) | scratch (16-byte rows) | cu_tokens | granted
-    nws = _plan_ws(N)
-    head = 16 * max_tokens
-    buf = torch.empty(head + nws + 4 * (2 * N + 1), dtype=torch.uint8, device=lengths.device)
-    at = buf.data_ptr()
-    cu = at + head + nws
-    check(lib().vm_paged_plan(p[0], p[1], p[2], ld, N, M, p[3], p[4], P, page_size, at if max_tokens else None, at + 8 * max_tokens if max_tokens else None,
-                              max_tokens, cu, cu + 4 * (N + 1), at + head, nws, stream()), name)
-    small = buf[head + nws:].view(_I32)
-    both = buf[:head].view(_I64)
-    return both[:max_tokens], both[max_tokens:], small[:N + 1], small[N + 1:]
+    dev = lengths.device
+    slots = torch.empty(max_tokens, dtype=_I64, device=dev)
+    positions = torch.empty(max_tokens, dtype=_I64, device=dev)
+    cu = torch.empty(N + 1, dtype=_I32, device=dev)
+    granted = torch.empty(N, dtype=_I32, device=dev)
+    nws = _plan_ws(N, max_tokens)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    check(lib().vm_paged_plan(p[0], p[1], p[2], ld, N, M, p[3], p[4], P, page_size, ptr(slots), ptr(positions), max_tokens, ptr(cu), ptr(granted), ptr(ws), nws,
+                              stream()), name)
+    return slots, positions, cu, granted
 
 
 def _check_pages(name, k_pages, v_pages, other):
