@@ -43,15 +43,12 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, bool capped) {
     v = plan_add(v, plan_dpp<0x142, 0xa>(v), capped);
     return plan_add(v, plan_dpp<0x143, 0xc>(v), capped);
 }
-// inclusive scans of one or two values over the workgroup; `before` (the sum of earlier calls) is added and moved on
-template <int THREADS> __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_t& before, bool capped) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v, capped);
-    if (lane == 63) sh[wave] = v;
-    __syncthreads();
+// inclusive scan over the workgroup out of the wave scans and the waves' sums in `sh`; `before` (the sum of earlier calls) is added and moved on
+template <int WAVES> __device__ __forceinline__ uint32_t plan_join(uint32_t v, const uint32_t* sh, uint32_t& before, bool capped) {
+    const int wave = threadIdx.x >> 6;
     uint32_t mine = before, all = before;
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) { const uint32_t x = sh[w]; if (w < wave) mine = plan_add(mine, x, capped); all = plan_add(all, x, capped); }
+    for (int w = 0; w < WAVES; ++w) { const uint32_t x = sh[w]; if (w < wave) mine = plan_add(mine, x, capped); all = plan_add(all, x, capped); }
     before = all;
     return plan_add(mine, v, capped);
 }
@@ -59,9 +56,10 @@ template <int THREADS> __device__ __forceinline__ uint32_t block_scan(uint32_t v
 // FUSED: rows and cu are LDS arrays (cu is written to memory as well)
 template <int THREADS, bool FUSED>
 __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int* cu, PlanRing* snap) {
-    __shared__ uint32_t sh[3][THREADS / 64];
+    constexpr int WAVES = THREADS / 64;
+    __shared__ uint32_t sh[3][WAVES];
     __shared__ int s_taken;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int head = p.ring[0], count = p.ring[1];
     const int64_t cap = (int64_t)p.M * p.s;
     uint32_t tok_before = 0, want_before = 0, back_before = 0;
@@ -75,13 +73,18 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
         }
         const int64_t t = n > 0 ? n : 0;
         __syncthreads();                                                   // (sh is free again, s_taken is set)
-        const uint32_t end = block_scan<THREADS>((uint32_t)min(t, (int64_t)PLAN_FULL), sh[0], tok_before, true);
+        const uint32_t tok = wave_scan((uint32_t)min(t, (int64_t)PLAN_FULL), true);
+        if (lane == 63) sh[0][wave] = tok;
+        __syncthreads();
+        const uint32_t end = plan_join<WAVES>(tok, sh[0], tok_before, true);
         const int have = (int)((L + p.s - 1) / p.s);
         const bool fits = n > 0 && L + t <= cap && end <= (uint32_t)p.max_tokens;
         const int want = fits ? (int)((L + t + p.s - 1) / p.s) - have : 0;
         const int back = n < 0 ? have : 0;
-        const uint32_t upto = block_scan<THREADS>((uint32_t)want, sh[1], want_before, false);       // (below 2^31: the host checks N * M)
-        const uint32_t back_upto = block_scan<THREADS>((uint32_t)back, sh[2], back_before, false);
+        const uint32_t ws = wave_scan((uint32_t)want, false), bs = wave_scan((uint32_t)back, false);       // (sums below 2^31: the host checks N * M)
+        if (lane == 63) { sh[1][wave] = ws; sh[2][wave] = bs; }
+        __syncthreads();
+        const uint32_t upto = plan_join<WAVES>(ws, sh[1], want_before, false), back_upto = plan_join<WAVES>(bs, sh[2], back_before, false);
         const bool ok = fits && (want == 0 || (int)upto <= count);
         const bool last = ok && want > 0;                                  // the accepted rows that need pages are a prefix: the largest upto is their sum
         if (last) atomicMax(&s_taken, (int)upto);
@@ -113,17 +116,24 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
 }
 __device__ __forceinline__ int ring_place(int64_t at, int P) { const int r = (int)(at % P); return r < 0 ? r + P : r; }
 
-// table rows and ring places: wave `wave` of `waves`
-__device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows, const PlanRing g, int wave, int waves) {
-    const int lane = threadIdx.x & 63;
-    for (int i = wave; i < p.N; i += waves) {
+// table rows and ring places, thread `tid` of `threads`: rows that take one page (a decode step's) one thread each, the others by groups of lanes that
+// cover a table row (a wave where it is longer)
+__device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows, const PlanRing g, int tid, int threads) {
+    for (int i = tid; i < p.N; i += threads) {
+        const PlanRow r = rows[i];
+        if (r.kind == 1 && r.cnt == 1) p.table[(int64_t)i * p.ld_table + (r.len + p.s - 1) / p.s] = p.free_pages[ring_place((int64_t)g.head + r.ofs, p.P)];
+    }
+    int lanes = 64;
+    while (lanes > 8 && lanes / 2 >= p.M) lanes >>= 1;
+    const int lane = tid & (lanes - 1);
+    for (int i = tid / lanes; i < p.N; i += threads / lanes) {
         const PlanRow r = rows[i];
         int32_t* row = p.table + (int64_t)i * p.ld_table;
-        if (r.kind == 1) {
+        if (r.kind == 1 && r.cnt > 1) {
             const int have = (r.len + p.s - 1) / p.s;
-            for (int j = lane; j < r.cnt; j += 64) row[have + j] = p.free_pages[ring_place((int64_t)g.head + r.ofs + j, p.P)];
+            for (int j = lane; j < r.cnt; j += lanes) row[have + j] = p.free_pages[ring_place((int64_t)g.head + r.ofs + j, p.P)];
         } else if (r.kind == 2) {
-            for (int j = lane; j < p.M; j += 64) {
+            for (int j = lane; j < p.M; j += lanes) {
                 if (j < r.cnt && r.ofs + j < g.returned) p.free_pages[ring_place((int64_t)g.head + g.count + r.ofs + j, p.P)] = row[j];
                 row[j] = -1;
             }
@@ -157,13 +167,13 @@ __global__ __launch_bounds__(THREADS) void paged_plan_step_kernel(const PlanArgs
     plan_scan<THREADS, true>(p, rows, cu, &snap);
     __syncthreads();
     const PlanRing g = snap;
-    plan_rows(p, rows, g, threadIdx.x >> 6, THREADS / 64);
+    plan_rows(p, rows, g, threadIdx.x, THREADS);
     for (int t = threadIdx.x; t < p.max_tokens; t += THREADS) plan_token(p, rows, cu, g, t);
 }
 __global__ __launch_bounds__(PLAN_THREADS) void paged_plan_scan_kernel(const PlanArgs p) { plan_scan<PLAN_THREADS, false>(p, p.rows, p.cu, p.snap); }
 __global__ __launch_bounds__(256) void paged_plan_fill_kernel(const PlanArgs p) {
     const PlanRing g = *p.snap;
-    plan_rows(p, p.rows, g, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
+    plan_rows(p, p.rows, g, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
     for (int t = blockIdx.x * 256 + threadIdx.x; t < p.max_tokens; t += gridDim.x * 256) plan_token(p, p.rows, p.cu, g, t);
 }
 
