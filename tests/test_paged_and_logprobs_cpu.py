@@ -124,3 +124,33 @@ def test_c_entries_refuse_without_touching_the_device():
     assert L.vm_paged_attention(fake, 8, 8, fake, fake, fake, 1, fake, fake, 1, 1, 1, 16, 1, 24, 1, 1.0, 1, None, 0, None) == -1
     assert L.vm_paged_plan(fake, fake, fake, 4, 2000, 4, fake, fake, 8, 16, fake, fake, 8, fake, fake, fake, 8, None) == -1      # workspace too small
     assert L.vm_paged_plan_ws(0, 5) == 0 and L.vm_paged_plan_ws(2000, 5) >= 2000 * 16
+
+
+def test_paged_cache_holds_its_tensors_and_refuses():
+    from vilmedic_amd.paged import PagedKVCache
+    c = PagedKVCache(2, 3, 4, 16, 33, dtype=torch.float32, device="cpu")
+    assert c.pages.shape == (2, 2, 9, 4, 16, 16) and c.block_table.shape == (3, 3) and c.free_ring.tolist() == [0, 9]
+    c.free_ring[0], c.free_ring[1], c.lengths[1] = 5, 2, 7
+    c.free_pages.fill_(3)
+    c.reset()
+    assert c.free_ring.tolist() == [0, 9] and c.free_pages.tolist() == list(range(9)) and not c.lengths.any() and bool((c.block_table == -1).all())
+    for bad in (dict(page_size=24), dict(page_size=8), dict(pages=0), dict(max_tokens=0), dict(rows=0), dict(layers=0)):
+        with pytest.raises(ValueError, match="PagedKVCache"):
+            PagedKVCache(**{**dict(layers=1, rows=2, heads=1, head_dim=16, max_tokens=20, device="cpu"), **bad})
+
+
+def test_generate_refuses_paged_caches_where_they_do_not_serve():
+    from vilmedic_amd.generation import generate
+
+    class Cfg:
+        eos_token_id, pad_token_id, bos_token_id = 2, 1, 0
+
+    class Dec:
+        config = Cfg()
+    ids, enc = torch.zeros(2, 1, dtype=torch.long), torch.zeros(2, 3, 8)
+    for kw, err in ((dict(kv_cache="pages"), ValueError), (dict(output_logprobs=3), ValueError), (dict(kv_cache="paged", num_beams=4), NotImplementedError),
+                    (dict(output_logprobs=3, num_beams=4, return_dict_in_generate=True), NotImplementedError)):
+        with pytest.raises(err):
+            generate(Dec(), input_ids=ids, encoder_hidden_states=enc, **kw)
+    with pytest.raises(NotImplementedError):
+        generate(Dec(), input_ids=ids, hf_models=[Dec(), Dec()], encoders_outputs=[dict(encoder_hidden_states=enc)] * 2, kv_cache="paged")

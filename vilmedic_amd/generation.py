@@ -30,6 +30,7 @@ from . import ops
 from ._lib import VM_BF16, VM_F32, DecodeGemmArgs, check, lib, ptr, stream
 from .arena import arena_of
 from .nn import to_key_mask
+from .paged import PagedKVCache
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -86,9 +87,13 @@ def _attn32(q, k, ldk, v, ldv, rows, H, Lk, dh, q_per_kv, key_mask=None, kv_inde
 class DecodeState:
     """Per-generate() state: cross K|V per layer, self K|V cache [rows*T, 2D] per layer, row-index table [rows, T]."""
 
-    def __init__(self, decoder, enc, enc_mask, beams, max_length, dtype="bf16"):
+    def __init__(self, decoder, enc, enc_mask, beams, max_length, dtype="bf16", paged=None):
+        """``paged``: None (one contiguous cache row of max_length per row) or (page_size, pages or None): the self-attention cache is a PagedKVCache
+        whose rows give their pages back when they finish (``alive``)"""
         if dtype not in ("bf16", "fp32"):
             raise ValueError(f"decode_dtype must be 'bf16' or 'fp32', got {dtype!r}")
+        if paged is not None and beams != 1:
+            raise NotImplementedError("a paged cache serves greedy decoding and sampling: a beam reorder would have to copy half-filled pages")
         self.f32 = dtype == "fp32"
         self.act = F32 if self.f32 else BF16
         self.dec = decoder
@@ -118,7 +123,14 @@ class DecodeState:
         # static buffers (their addresses are baked into the captured graphs)
         self.enc_mask = torch.ones(self.B, self.S, dtype=torch.uint8, device=dev) if enc_mask is not None else None
         self.cross_kv = [torch.empty(self.B * self.S, 2 * self.Da, dtype=self.act, device=dev) for _ in self.layers]
-        self.self_kv = [torch.empty(self.M * self.T, 2 * self.Da, dtype=self.act, device=dev) for _ in self.layers]
+        self.paged = None
+        if paged is not None:
+            self.paged = PagedKVCache(len(self.layers), self.M, self.H, self.dhp, self.T, page_size=paged[0], pages=paged[1], dtype=self.act, device=dev)
+            self.buf_kv = torch.empty(self.M, 2 * self.Da, dtype=self.act, device=dev)        # K|V of the new tokens, one row each
+            self.slots = torch.empty(self.M, dtype=torch.long, device=dev)
+            self.alive = None                 # uint8 / bool [M]: rows that still decode (None: all of them); set by the driver
+            self.starved = torch.zeros(self.M, dtype=torch.bool, device=dev)
+        self.self_kv = [None if paged is not None else torch.empty(self.M * self.T, 2 * self.Da, dtype=self.act, device=dev) for _ in self.layers]
         self.pw = None                    # per layer: the padded weights / biases of a padded-head step (built by load_encoder)
         self.index = torch.empty(self.M, self.T, dtype=torch.int32, device=dev)
         self.tok = torch.zeros(self.M, dtype=torch.long, device=dev)
@@ -145,10 +157,14 @@ class DecodeState:
         self.load_encoder(enc, enc_mask)
 
     def load_encoder(self, enc, enc_mask):
-        """(re)start a generation on this state: project the image features to every layer's cross K|V (once, shared by all
+        """(re)start a generation on this state: empty the paged cache, project the image features to every layer's cross K|V (once, shared by all
         beams of a sample), reset the row-index table.  Buffers keep their addresses, so captured graphs stay valid."""
         a = self.arena
         a.refresh()
+        if self.paged is not None:
+            self.paged.reset()
+            self.starved.zero_()
+            self.alive = None
         if self.pos_table is not None:
             e = self.dec.bert.embeddings
             with torch.no_grad():
@@ -213,6 +229,8 @@ class DecodeState:
     @torch.no_grad()
     def step(self, tokens, t):
         """tokens int64 [M] at position t  ->  fp32 logits [M, V] for position t+1 (valid until the next step(.., t))."""
+        if self.paged is not None:
+            self._plan()                      # outside the captured step: a graph's warm-up pass must not take pages
         if not DECODE_GRAPH:
             return self._step(tokens, t)
         self.tok.copy_(tokens)
@@ -230,6 +248,34 @@ class DecodeState:
             entry = self.graphs[t] = (graph, out)
         entry[0].replay()
         return entry[1]
+
+    def _plan(self):
+        """one more token for every row that still decodes, the pages of the others go back; the slots of the rows' tokens -> self.slots"""
+        if self.alive is None:
+            new = torch.ones(self.M, dtype=torch.int32, device=self.slots.device)
+        else:
+            new = self.alive.to(torch.int32) * 2 - 1                          # 1: one token, -1: release (nothing happens to an empty row)
+        slots, _, cu, granted = self.paged.plan(new, self.M)
+        got = granted > 0
+        self.starved |= (new > 0) & ~got
+        self.slots.copy_(torch.where(got, slots[cu[:-1].clamp(max=self.M - 1).long()], torch.full_like(slots, -1)))
+
+    def check_pages(self):
+        """(host sync) the pool has had a page for every token so far"""
+        if self.paged is not None and bool(self.starved.any()):
+            raise RuntimeError(f"generate(kv_cache='paged'): {self.paged.free_pages.shape[0]} pages of {self.paged.page_size} tokens do not hold this batch; "
+                               "raise kv_pages")
+
+    def _self_attention(self, li, q, t, Da, dh, scale=None):
+        """attention of the new tokens over their rows' histories (K|V of the new tokens are in the cache, or in buf_kv of a paged one)"""
+        if self.paged is not None:
+            M, H = self.M, self.H
+            self.paged.write(li, self.buf_kv[:, :Da].view(M, H, dh), self.buf_kv[:, Da:].unflatten(1, (H, dh)), self.slots)
+            return self.paged.attend(li, q[:, :Da].unflatten(1, (H, dh)), scale if scale is not None else dh ** -0.5).view(M, Da)
+        cache = self.self_kv[li]
+        if self.f32:
+            return _attn32(q, cache, 2 * Da, cache[:, Da:], 2 * Da, self.M, self.H, t + 1, dh, 1, kv_index=self.index, kv_index_ld=self.T, scale=scale)
+        return _attn(q, q.stride(0), cache, 2 * Da, cache[:, Da:], 2 * Da, self.M, self.H, 1, t + 1, dh, kv_index=self.index, kv_index_ld=self.T, scale=scale)
 
     # ---- one decode step = embedding + 8 launches per layer + final LayerNorm + LM head (csrc/decode_gemm.hip: every LayerNorm but the
     # last is computed by the projection that consumes it, Q|K|V is one projection with two destinations)
@@ -316,15 +362,15 @@ class DecodeState:
         Da, dhp, sc = self.Da, self.dhp, self.scale
         for li, layer in enumerate(self.layers):
             sa = layer.attention.self
-            cache = self.self_kv[li]
+            if self.paged is not None:           # K|V of the new tokens: rows of a buffer, written into the pages from there
+                new_kv, new_ld = self.buf_kv, 2 * Da
+            else:                                # ... or their rows of the cache
+                new_kv, new_ld = self.self_kv[li][t:], T * 2 * Da
             if self.padded:                      # the same eight launches on the zero-padded projections (load_encoder built them)
                 pw = self.pw[li]
                 qp = q[:, :Da] if q.shape[1] == Da else q.as_strided((M, Da), (q.stride(0), 1))
-                self._dgl(s, ln, x, pw["qkv"][0], qp, M, 3 * Da, D, bias=pw["qkv"][1], c2=cache[t:], ldc2=T * 2 * Da, split_n=Da)
-                if self.f32:
-                    ctx = _attn32(qp, cache, 2 * Da, cache[:, Da:], 2 * Da, M, H, t + 1, dhp, 1, kv_index=self.index, kv_index_ld=T, scale=sc)
-                else:
-                    ctx = _attn(qp, qp.stride(0), cache, 2 * Da, cache[:, Da:], 2 * Da, M, H, 1, t + 1, dhp, kv_index=self.index, kv_index_ld=T, scale=sc)
+                self._dgl(s, ln, x, pw["qkv"][0], qp, M, 3 * Da, D, bias=pw["qkv"][1], c2=new_kv, ldc2=new_ld, split_n=Da)
+                ctx = self._self_attention(li, qp, t, Da, dhp, sc)
                 blk = layer.attention.output
                 self._dg(ctx, pw["so"], s, M, D, Da, bias=blk.dense.bias, residual=x)
                 self._dgl(s, blk.LayerNorm, x, pw["cq"][0], qp, M, Da, D, bias=pw["cq"][1])
@@ -344,15 +390,12 @@ class DecodeState:
                 continue
             if getattr(sa, "fuse_q", False):     # Q|K|V in one launch: Q -> q, K|V of the new token -> cache row t
                 self._dgl(s, ln, x, self._w([sa.query.weight, sa.key.weight, sa.value.weight]), q, M, 3 * D, D,
-                          bias=a.f32_group([sa.query.bias, sa.key.bias, sa.value.bias]), c2=cache[t:], ldc2=T * 2 * D, split_n=D)
+                          bias=a.f32_group([sa.query.bias, sa.key.bias, sa.value.bias]), c2=new_kv, ldc2=new_ld, split_n=D)
             else:
                 self._dgl(s, ln, x, self._w([sa.query.weight]), q, M, D, D, bias=sa.query.bias)
-                self._dg(x, self._w([sa.key.weight, sa.value.weight]), cache[t:].as_strided((M, 2 * D), (T * 2 * D, 1)), M, 2 * D, D,
+                self._dg(x, self._w([sa.key.weight, sa.value.weight]), new_kv.as_strided((M, 2 * D), (new_ld, 1)), M, 2 * D, D,
                          bias=a.f32_group([sa.key.bias, sa.value.bias]))
-            if self.f32:
-                ctx = _attn32(q, cache, 2 * D, cache[:, D:], 2 * D, M, H, t + 1, D // H, 1, kv_index=self.index, kv_index_ld=T)
-            else:
-                ctx = _attn(q, D, cache, 2 * D, cache[:, D:], 2 * D, M, H, 1, t + 1, D // H, kv_index=self.index, kv_index_ld=T)
+            ctx = self._self_attention(li, q, t, D, D // H)
             blk = layer.attention.output
             self._dg(ctx, self._w([blk.dense.weight]), s, M, D, D, bias=blk.dense.bias, residual=x)
             ca = layer.crossattention.self
@@ -413,29 +456,31 @@ class EnsembleState:
 _STATE_CACHE = weakref.WeakKeyDictionary()
 
 
-def _cached_state(decoder, enc, enc_mask, beams, max_length, dtype="bf16"):
+def _cached_state(decoder, enc, enc_mask, beams, max_length, dtype="bf16", paged=None):
     """decode states (KV caches, cross K|V buffers, captured graphs) live on the decoder and are reused by generate()
     calls of the same shape; the key includes the arena's shadow buffer so a re-flattened model starts afresh"""
     if not DECODE_GRAPH:
-        return DecodeState(decoder, enc, enc_mask, beams, max_length, dtype)
+        return DecodeState(decoder, enc, enc_mask, beams, max_length, dtype, paged)
     cache = _STATE_CACHE.setdefault(decoder, {})        # weak: dies with the decoder; never part of deepcopy / pickling of the model
     arena = arena_of(decoder)
-    key = (enc.shape[0], enc.shape[1], enc.shape[2], beams, max_length, enc_mask is not None, arena.shadow_flat.data_ptr(), str(enc.device), dtype)
+    key = (enc.shape[0], enc.shape[1], enc.shape[2], beams, max_length, enc_mask is not None, arena.shadow_flat.data_ptr(), str(enc.device), dtype, paged)
     st = cache.get(key)
     if st is None:
         if len(cache) >= 4:
             cache.clear()
-        st = cache[key] = DecodeState(decoder, enc, enc_mask, beams, max_length, dtype)
+        st = cache[key] = DecodeState(decoder, enc, enc_mask, beams, max_length, dtype, paged)
     else:
         st.load_encoder(enc, enc_mask)
     return st
 
 
-def _decode_state(decoder, enc, enc_mask, beams, max_length, dtype=None):
+def _decode_state(decoder, enc, enc_mask, beams, max_length, dtype=None, paged=None):
     dtype = dtype or DECODE_DTYPE
     if isinstance(decoder, (list, tuple)):
+        if paged is not None:
+            raise NotImplementedError("ensembles decode on contiguous caches")
         return EnsembleState(decoder, enc, enc_mask, beams, max_length, dtype), decoder[0], enc[0]
-    return _cached_state(decoder, enc, enc_mask, beams, max_length, dtype), decoder, enc
+    return _cached_state(decoder, enc, enc_mask, beams, max_length, dtype, paged), decoder, enc
 
 
 def log_softmax_f32(logits):
@@ -453,8 +498,8 @@ def argmax_f32(x):
 
 
 class GenerateOutput:
-    def __init__(self, sequences, sequences_scores=None, scores=None):
-        self.sequences, self.sequences_scores, self.scores = sequences, sequences_scores, scores
+    def __init__(self, sequences, sequences_scores=None, scores=None, logprobs=None):
+        self.sequences, self.sequences_scores, self.scores, self.logprobs = sequences, sequences_scores, scores, logprobs
 
 
 def _process(logits, bad_ids, top_k):
@@ -480,13 +525,16 @@ def trim_to_last_eos(seq, eos_token_id):
 
 
 def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_token_id, do_sample=False, top_k=None,
-           bad_words_ids=None, output_scores=False, generator=None, decode_dtype=None, greedy_rows=None):
+           bad_words_ids=None, output_scores=False, generator=None, decode_dtype=None, greedy_rows=None, output_logprobs=None, paged=None):
     """HF ``_sample``: greedy (argmax) or multinomial sampling, 1 sequence per batch row.  ``greedy_rows`` = n (with do_sample):
     the first n rows decode greedily on the RAW logits, the others sample from the processed ones -- two rollouts in one pass of
     launch-latency-bound decode steps (SCST: baseline + sampled rollout); callers split the rows and trim each part
-    (trim_to_last_eos)."""
+    (trim_to_last_eos).  ``output_logprobs`` = k: ops.TokenLogprobs of the emitted tokens (position j of each field belongs to sequences[:, j + 1]) under
+    the model's own distribution -- before bad words and top-k -- with its entropy and k best alternatives; finished rows hold zeros.
+    ``paged`` = (page_size, pages or None): decode on a paged cache (DecodeState)."""
     B = input_ids.shape[0]
-    st, decoder, enc0 = _decode_state(decoder, enc, enc_mask, 1, max_length, decode_dtype)
+    st, decoder, enc0 = _decode_state(decoder, enc, enc_mask, 1, max_length, decode_dtype, paged)
+    logprobs = []
     dev = enc0.device
     seq = torch.full((B, max_length), pad_token_id, dtype=torch.long, device=dev)
     seq[:, 0] = input_ids[:, 0]
@@ -499,6 +547,8 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
         V = decoder.config.vocab_size
         g_rows = (int(greedy_rows) if greedy_rows else 0) if do_sample else B
         unf = torch.ones(B, dtype=torch.uint8, device=dev)
+        if paged is not None:
+            st.alive = unf
         nxt = torch.empty(B, dtype=torch.long, device=dev)
         ban = (C_.c_int32 * 4)(*(bad + [0] * (4 - len(bad)))) if bad else None
         # the draws follow torch's seeding (torch.manual_seed / an explicit CPU generator) through ONE host-side draw per call
@@ -511,6 +561,8 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
             logits = st.step(seq[:, cur - 1], cur - 1)
             check(lib().vm_select_tokens(ptr(logits), logits.stride(0), B, V, g_rows, ban, len(bad), int(top_k or 0) if do_sample else 0, seed, ptr(nxt),
                                          ptr(seq), seq.stride(0), cur, ptr(unf), eos_token_id, pad_token_id, stream()), "vm_select_tokens")
+            if output_logprobs is not None:
+                logprobs.append(ops.token_logprobs(logits, nxt, output_logprobs))
             cur += 1
             if cur % 8 == 0 and not bool(unf.any()):           # host sync only every 8 steps; trimmed exactly below
                 break
@@ -521,7 +573,9 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
     # ``greedy_rows`` keeps its meaning: the first rows take the arg-max of the RAW logits).
     unfinished = torch.ones(B, dtype=torch.bool, device=dev)
     while not fused and cur < max_length:
-        logits = st.step(seq[:, cur - 1], cur - 1)
+        if paged is not None:
+            st.alive = unfinished
+        raw = logits = st.step(seq[:, cur - 1], cur - 1)
         if do_sample and greedy_rows:
             g = int(greedy_rows)
             nxt = torch.empty(B, dtype=torch.long, device=dev)
@@ -540,11 +594,15 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
         if output_scores:
             scores.append(logits)
         nxt = torch.where(unfinished, nxt, torch.full_like(nxt, pad_token_id))
+        if output_logprobs is not None:
+            logprobs.append(ops.token_logprobs(raw, nxt, output_logprobs))
         seq[:, cur] = nxt
         unfinished = unfinished & (nxt != eos_token_id)
         cur += 1
         if cur % 8 == 0 and not bool(unfinished.any()):      # host sync only every 8 steps; trimmed exactly below
             break
+    if paged is not None:
+        st.check_pages()
     # exact HF stopping point: generation ends right after the step at which the last row finished
     seq = seq[:, :cur]
     is_eos = seq[:, 1:] == eos_token_id
@@ -552,7 +610,21 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
         last = int((is_eos.float().argmax(dim=1) + 1).max()) + 1
         seq = seq[:, :last]
         scores = scores[:last - 1]
-    return GenerateOutput(seq, None, tuple(scores) if output_scores else None)
+    if output_logprobs is not None:
+        logprobs = _emitted_logprobs(logprobs, seq, eos_token_id, output_logprobs)
+    return GenerateOutput(seq, None, tuple(scores) if output_scores else None, logprobs if output_logprobs is not None else None)
+
+
+def _emitted_logprobs(steps, seq, eos_token_id, top):
+    """the steps' TokenLogprobs as [B, length - 1] fields; what follows a row's first eos was not decoded: zeros"""
+    B, n = seq.shape[0], seq.shape[1] - 1
+    if n == 0:
+        f = torch.zeros(B, 0, dtype=torch.float32, device=seq.device)
+        return ops.TokenLogprobs(f, f.clone(), f.new_zeros(B, 0, top), torch.zeros(B, 0, top, dtype=torch.long, device=seq.device))
+    fields = [torch.stack(f, 1) for f in zip(*steps[:n])]
+    is_eos = (seq[:, 1:] == eos_token_id).long()
+    gone = (torch.cumsum(is_eos, 1) - is_eos) > 0
+    return ops.TokenLogprobs(*(f.masked_fill(gone if f.dim() == 2 else gone[..., None], 0) for f in fields))
 
 
 def _gather(t, idx):
@@ -646,6 +718,15 @@ def generate(decoder, input_ids=None, encoder_hidden_states=None, encoder_attent
     pad = args.get("pad_token_id", cfg.pad_token_id)
     nb = args.get("num_beams") or 1
     ret_dict = args.get("return_dict_in_generate", False)
+    # ``kv_cache="paged"`` (``kv_page_size`` tokens per page, ``kv_pages`` in all; default: enough for every row at max_length): rows that finish give their
+    # memory back.  ``output_logprobs=k``: GenerateOutput.logprobs (sample()).
+    paged = None
+    if args.get("kv_cache") not in (None, "contiguous"):
+        if args["kv_cache"] != "paged":
+            raise ValueError(f"kv_cache must be 'contiguous' or 'paged', got {args['kv_cache']!r}")
+        paged = (int(args.get("kv_page_size") or 16), None if args.get("kv_pages") is None else int(args["kv_pages"]))
+    if args.get("output_logprobs") is not None and not ret_dict:
+        raise ValueError("output_logprobs needs return_dict_in_generate=True")
     if input_ids is None:
         bos = args.get("bos_token_id", cfg.bos_token_id)
         e0 = encoder_hidden_states[0] if isinstance(encoder_hidden_states, (list, tuple)) else encoder_hidden_states
@@ -655,6 +736,8 @@ def generate(decoder, input_ids=None, encoder_hidden_states=None, encoder_attent
     if nb > 1:
         if args.get("do_sample"):
             raise NotImplementedError("beam sampling is outside the reference's call sites")
+        if paged is not None or args.get("output_logprobs") is not None:
+            raise NotImplementedError("kv_cache='paged' and output_logprobs serve greedy decoding and sampling, not beam search")
         out = beam_search(decoder, input_ids, encoder_hidden_states, encoder_attention_mask, max_length=max_length,
                           eos_token_id=eos, pad_token_id=pad, num_beams=nb, length_penalty=args.get("length_penalty", 1.0) or 1.0,
                           decode_dtype=args.get("decode_dtype"))
@@ -662,5 +745,6 @@ def generate(decoder, input_ids=None, encoder_hidden_states=None, encoder_attent
         out = sample(decoder, input_ids, encoder_hidden_states, encoder_attention_mask, max_length=max_length, eos_token_id=eos,
                      pad_token_id=pad, do_sample=bool(args.get("do_sample")), top_k=args.get("top_k"),
                      bad_words_ids=args.get("bad_words_ids"), output_scores=bool(args.get("output_scores")),
-                     generator=args.get("generator"), decode_dtype=args.get("decode_dtype"), greedy_rows=args.get("greedy_rows"))
+                     generator=args.get("generator"), decode_dtype=args.get("decode_dtype"), greedy_rows=args.get("greedy_rows"),
+                     output_logprobs=args.get("output_logprobs"), paged=paged)
     return out if ret_dict else out.sequences
