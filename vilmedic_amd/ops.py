@@ -1272,14 +1272,13 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
     -> (slots int64 [max_tokens], positions int64 [max_tokens], cu_tokens int32 [N + 1], granted int32 [N]): where the packed new tokens go
     (-1: nowhere), their positions in their requests, the packed offsets of the rows, and the tokens each row was given."""
     name = "paged_plan"
-    for what, t, nd in (("lengths", lengths, 1), ("new_tokens", new_tokens, 1), ("block_table", block_table, 2), ("free_pages", free_pages, 1),
-                        ("free_ring", free_ring, 1)):
-        if t.dtype != _I32 or t.dim() != nd:
-            _refuse(name, f"{what} must be an int32 tensor of {nd} dimension(s), got {_desc(t)}")
-        if t.device != lengths.device:
-            _refuse(name, f"all tensors must be on one device, got {lengths.device} and {t.device}")
-        if nd == 1 and not t.is_contiguous():
-            _refuse(name, f"{what} must be contiguous")
+    dev = lengths.device
+    if not (lengths.dtype == new_tokens.dtype == block_table.dtype == free_pages.dtype == free_ring.dtype == _I32
+            and lengths.dim() == new_tokens.dim() == free_pages.dim() == free_ring.dim() == 1 and block_table.dim() == 2
+            and new_tokens.device == dev and block_table.device == dev and free_pages.device == dev and free_ring.device == dev
+            and lengths.is_contiguous() and new_tokens.is_contiguous() and free_pages.is_contiguous() and free_ring.is_contiguous()):
+        _refuse(name, "lengths, new_tokens, free_pages and free_ring must be contiguous int32 vectors and block_table an int32 matrix, on one device; got "
+                + ", ".join(_desc(t) for t in (lengths, new_tokens, free_pages, free_ring, block_table)))
     N, M = block_table.shape
     P = free_pages.shape[0]
     page_size, max_tokens = int(page_size), int(max_tokens)
@@ -1296,8 +1295,7 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
         _refuse(name, f"max_tokens must lie between 0 and 2^30, got {max_tokens}")
     if N * M >= 1 << 31 or M * page_size >= 1 << 31:
         _refuse(name, "the table's size and M * page_size must stay below 2^31")
-    p = [ptr(t) for t in (lengths, new_tokens, block_table, free_pages, free_ring)]
-    dev = lengths.device
+    p = (ptr(lengths), ptr(new_tokens), ptr(block_table), ptr(free_pages), ptr(free_ring))
     slots = torch.empty(max_tokens, dtype=_I64, device=dev)
     positions = torch.empty(max_tokens, dtype=_I64, device=dev)
     cu = torch.empty(N + 1, dtype=_I32, device=dev)
