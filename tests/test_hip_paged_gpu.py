@@ -246,6 +246,18 @@ def test_attention_with_a_wide_table_of_short_rows_and_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Hq,H,dh,M", [(2, 2, 64, 8), (6, 2, 32, 8), (4, 2, 128, 100), (34, 1, 40, 8), (2, 2, 200, 8)])
+def test_attention_of_so_many_rows_that_one_wave_serves_each(dtype, Hq, H, dh, M):
+    N = 1600 if H == 2 else 1100                       # (34 query heads of one key head: three blocks of up to 16)
+    lens = [(i * 53) % 129 for i in range(N)]
+    if M == 100:
+        lens[7], lens[900] = 1600, 1111
+    k, v, table, lengths = make_cache(dtype, H, dh, 16, lens, seed=dh, M=M)
+    q = torch.randn(N, Hq, dh, generator=torch.Generator().manual_seed(2)).to(dtype)
+    check_attention(q, k, v, table, lengths)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_strides_of_q_and_table(dtype):
     from vilmedic_amd import ops
     lens = [40, 3, 129]

@@ -236,6 +236,21 @@ def test_gradient_agrees_with_differences():
         assert abs(xd.grad[r, c].item() - want.item()) <= 1e-5 + 1e-5 * abs(want.item())
 
 
+def test_second_derivatives_are_refused_and_in_place_changes_noticed():
+    from vilmedic_amd import ops
+    x = torch.randn(3, 50, device=dev(), requires_grad=True)
+    t = torch.tensor([1, 2, 3], device=dev())
+    g = torch.autograd.grad(ops.token_logprobs(x, t).logp.sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    y = x * 1.0
+    out = ops.token_logprobs(y, t)
+    out.logp.mul_(2.0)                                   # outputs are tensors of their own
+    y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logp.sum().backward()
+
+
 def test_each_gradient_alone_and_none():
     from vilmedic_amd import ops
     x, t, _ = make(6, 300, F32, seed=10)

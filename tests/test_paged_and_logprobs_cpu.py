@@ -123,7 +123,7 @@ def test_c_entries_refuse_without_touching_the_device():
     assert L.vm_paged_attention(fake, 8, 8, fake, fake, fake, 1, fake, fake, 1, 1, 1, 12, 1, 16, 1, 1.0, 1, None, 0, None) == -1
     assert L.vm_paged_attention(fake, 8, 8, fake, fake, fake, 1, fake, fake, 1, 1, 1, 16, 1, 24, 1, 1.0, 1, None, 0, None) == -1
     assert L.vm_paged_plan(fake, fake, fake, 4, 2000, 4, fake, fake, 8, 16, fake, fake, 8, fake, fake, fake, 8, None) == -1      # workspace too small
-    assert L.vm_paged_plan_ws(0, 5) == 0 and L.vm_paged_plan_ws(2000, 5) >= 2000 * 16
+    assert L.vm_paged_plan_ws(0, 4, 5) == 0 and L.vm_paged_plan_ws(64, 16, 64) == 0 and L.vm_paged_plan_ws(2000, 4, 5) >= 2000 * 16
 
 
 def test_paged_cache_holds_its_tensors_and_refuses():

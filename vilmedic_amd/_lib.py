@@ -124,7 +124,7 @@ SIGNATURES = {
     "vm_gemm_f32": (_I, [_P, _L, _P, _L, _P, _L, _I, _I, _I, _P, _I, _P, _L, _P]),
     "vm_layernorm_f32": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
     "vm_embedding_fwd_f32": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
-    "vm_paged_plan_ws": (_SZ, [_I, _I]),
+    "vm_paged_plan_ws": (_SZ, [_I, _I, _I]),
     "vm_paged_plan": (_I, [_P, _P, _P, _L, _I, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "vm_paged_kv_write": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "vm_paged_attention_ws": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
@@ -171,6 +171,13 @@ def stream():
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())          # (a plain int: ctypes converts it for a c_void_p parameter itself)
     return torch.cuda.current_stream().cuda_stream
+
+
+def stream_on(index):
+    """raw hipStream_t of torch's current stream on device ``index``"""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def ptr(t):

@@ -20,7 +20,7 @@
 // (binary search of the row in the token offsets).  A step of a running batch does both in ONE launch of one workgroup, with everything that B needs
 // in LDS; with more rows or tokens B is a launch of its own over the chip.
 struct PlanRow { int len, ofs, cnt, kind; };       // kind 0 refused / nothing, 1 accepted (cnt pages from ring place head + ofs), 2 released (cnt pages back)
-struct PlanRing { int head, count, returned, pad; };
+struct PlanRing { int head, count, returned, more; };      // more: rows that take several pages or return some
 struct PlanArgs {
     int32_t* lengths; const int32_t* new_tokens; int32_t* table; int64_t ld_table; int N, M; int32_t* free_pages; int32_t* ring; int P, s;
     int64_t* slots; int64_t* positions; int max_tokens; int32_t* cu; int32_t* granted; PlanRow* rows; PlanRing* snap;
@@ -28,6 +28,7 @@ struct PlanArgs {
 #define PLAN_THREADS 1024
 #define PLAN_FUSED_ROWS 1024
 #define PLAN_FUSED_TOKENS 4096
+#define PLAN_FUSED_TABLE 65536
 #define PLAN_FULL ((1u << 30) + 1)                // token sums stop here: past every max_tokens, and two of them fit into 32 bits
 
 // inclusive scan over the wave: rows of 16 lanes first (row_shr 1, 2, 4, 8), then lane 15 of each row into the next (row_bcast15, row_bcast31)
@@ -58,12 +59,12 @@ template <int THREADS, bool FUSED>
 __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int* cu, PlanRing* snap) {
     constexpr int WAVES = THREADS / 64;
     __shared__ uint32_t sh[3][WAVES];
-    __shared__ int s_taken;
+    __shared__ int s_taken, s_more;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int head = p.ring[0], count = p.ring[1];
+    const int head = (p.ring[0] % p.P + p.P) % p.P, count = min(max(p.ring[1], 0), p.P);      // (outside: the caller's error, and no way out of the ring)
     const int64_t cap = (int64_t)p.M * p.s;
     uint32_t tok_before = 0, want_before = 0, back_before = 0;
-    if (tid == 0) s_taken = 0;
+    if (tid == 0) s_taken = s_more = 0;
     for (int base = 0; base < p.N; base += THREADS) {
         const int i = base + tid;
         int64_t L = 0; int n = 0;
@@ -95,6 +96,7 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
             r.cnt = n < 0 ? back : (ok ? want : 0);
             r.ofs = n < 0 ? (int)back_upto - back : (int)upto - want;
             rows[i] = r;
+            if (r.kind == 2 || r.cnt > 1) s_more = 1;
             p.lengths[i] = n < 0 ? 0 : (int)(L + (ok ? t : 0));
             p.granted[i] = ok ? (int)t : 0;
             const int e = (int)min(end, (uint32_t)p.max_tokens);
@@ -106,15 +108,15 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
     if (tid == 0) {
         cu[0] = 0;
         if constexpr (FUSED) p.cu[0] = 0;
-        const int64_t room = (int64_t)p.P - count;                        // (a count that lies outside [0, P] is the caller's error; nothing is read or written outside)
-        const int returned = (int)((int64_t)back_before < room ? (int64_t)back_before : (room > 0 ? room : 0));
-        PlanRing g = {head, count, returned, 0};
+        const int returned = min((int)back_before, p.P - count);           // (more than fits: pages returned twice, the caller's error)
+        PlanRing g = {head, count, returned, s_more};
         *snap = g;
         p.ring[0] = (int)(((int64_t)head + s_taken) % p.P);
         p.ring[1] = count - s_taken + returned;
     }
 }
-__device__ __forceinline__ int ring_place(int64_t at, int P) { const int r = (int)(at % P); return r < 0 ? r + P : r; }
+// head + something below 2 P, taken around the ring (no division: a 64-bit one costs more than everything around it)
+__device__ __forceinline__ int ring_place(int64_t at, int P) { at -= at >= P ? P : 0; return (int)(at - (at >= P ? P : 0)); }
 
 // table rows and ring places, thread `tid` of `threads`: rows that take one page (a decode step's) one thread each, the others by groups of lanes that
 // cover a table row (a wave where it is longer)
@@ -123,6 +125,7 @@ __device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows
         const PlanRow r = rows[i];
         if (r.kind == 1 && r.cnt == 1) p.table[(int64_t)i * p.ld_table + (r.len + p.s - 1) / p.s] = p.free_pages[ring_place((int64_t)g.head + r.ofs, p.P)];
     }
+    if (!g.more) return;
     int lanes = 64;
     while (lanes > 8 && lanes / 2 >= p.M) lanes >>= 1;
     const int lane = tid & (lanes - 1);
@@ -177,8 +180,10 @@ __global__ __launch_bounds__(256) void paged_plan_fill_kernel(const PlanArgs p) 
     for (int t = blockIdx.x * 256 + threadIdx.x; t < p.max_tokens; t += gridDim.x * 256) plan_token(p, p.rows, p.cu, g, t);
 }
 
-static bool plan_fused(int N, int max_tokens) { return N <= PLAN_FUSED_ROWS && max_tokens <= PLAN_FUSED_TOKENS; }
-extern "C" size_t vm_paged_plan_ws(int N, int max_tokens) { return N <= 0 || plan_fused(N, max_tokens) ? 0 : (size_t)N * sizeof(PlanRow) + sizeof(PlanRing); }
+// One launch while one workgroup can do the step: its rows fit into LDS, and the tokens do not keep it busy for long.  500 rows x 128 columns: one more token for
+// each in one launch 6.3 us, in two 8.5 us and 5 us more of the host; releasing all of them at once 24 us against 8.5, which is rarer.
+static bool plan_fused(int N, int M, int max_tokens) { return N <= PLAN_FUSED_ROWS && max_tokens <= PLAN_FUSED_TOKENS && (int64_t)N * M <= PLAN_FUSED_TABLE; }
+extern "C" size_t vm_paged_plan_ws(int N, int M, int max_tokens) { return N <= 0 || plan_fused(N, M, max_tokens) ? 0 : (size_t)N * sizeof(PlanRow) + sizeof(PlanRing); }
 
 extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int64_t ld_table, int N, int M, int32_t* free_pages,
                              int32_t* ring, int P, int page_size, int64_t* slots, int64_t* positions, int max_tokens, int32_t* cu_tokens,
@@ -188,14 +193,14 @@ extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_
     VM_REQUIRE(max_tokens == 0 || (slots && positions), "vm_paged_plan: slots and positions of max_tokens entries required");
     VM_REQUIRE(max_tokens <= (1 << 30), "vm_paged_plan: max_tokens must be at most 2^30");
     VM_REQUIRE((int64_t)N * M < (1ll << 31) && (int64_t)M * page_size < (1ll << 31), "vm_paged_plan: N * M and M * page_size must stay below 2^31");
-    const size_t need = vm_paged_plan_ws(N, max_tokens);
+    const size_t need = vm_paged_plan_ws(N, M, max_tokens);
     VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_plan: 16-byte aligned workspace of %zu bytes required", need);
     PlanRow* rows = reinterpret_cast<PlanRow*>(ws);
     PlanArgs a = {lengths, new_tokens, block_table, ld_table, N, M, free_pages, ring, P, page_size, slots, positions, max_tokens, cu_tokens, granted,
                   rows, reinterpret_cast<PlanRing*>(rows + N)};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_DECODE, 16.0 * N + 16.0 * max_tokens, s, "paged_plan_n%d_t%d", N, max_tokens);
-    if (plan_fused(N, max_tokens)) {
+    if (plan_fused(N, M, max_tokens)) {
         if (N <= 256 && max_tokens <= 1024) hipLaunchKernelGGL(paged_plan_step_kernel<256>, dim3(1), dim3(256), 0, s, a);
         else hipLaunchKernelGGL(paged_plan_step_kernel<1024>, dim3(1), dim3(1024), 0, s, a);
         return vm_check_launch("vm_paged_plan");

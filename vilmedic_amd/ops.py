@@ -19,9 +19,10 @@ import os
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import GemmEpilogue, VM_BF16, VM_F32, check, lib, ptr, stream
+from ._lib import GemmEpilogue, VM_BF16, VM_F32, check, lib, ptr, stream, stream_on
 
 BF16 = torch.bfloat16
 
@@ -1226,16 +1227,12 @@ _DT = {torch.float32: VM_F32, BF16: VM_BF16}
 _I32, _I64 = torch.int32, torch.int64
 
 
-def _on_device_of(fn):
-    """launch on the device (and its current stream) that the call's tensors live on, whichever device is current"""
-    @functools.wraps(fn)
-    def call(*args, **kw):
-        t = args[0] if args else next((x for x in kw.values() if isinstance(x, torch.Tensor)), None)
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
-                return fn(*args, **kw)
-        return fn(*args, **kw)
-    return call
+def _elsewhere(t):
+    """None when ``t`` lives on the current device, else the context that makes its device current (a launch goes to the current device)"""
+    dev = t.get_device()
+    if dev < 0:
+        ptr(t)                           # raises: there is no CPU fallback
+    return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _refuse(name, why):
@@ -1246,14 +1243,9 @@ def _desc(t):
     return f"{tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}"
 
 
-def _need_inference(name, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        _refuse(name, "it has no backward pass: call it under torch.no_grad()")
-
-
 @functools.lru_cache(maxsize=1024)
-def _plan_ws(N, max_tokens):
-    return lib().vm_paged_plan_ws(N, max_tokens)
+def _plan_ws(N, M, max_tokens):
+    return lib().vm_paged_plan_ws(N, M, max_tokens)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1261,7 +1253,6 @@ def _attention_ws(N, Hq, H, dh, M, s, dt):
     return lib().vm_paged_attention_ws(N, Hq, H, dh, M, s, dt)
 
 
-@_on_device_of
 def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_size, max_tokens):
     """Admit, grow and release the requests of a paged cache on the device (vm_paged_plan).
 
@@ -1293,17 +1284,21 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
         _refuse(name, "at least one row, one column, one page and one token per page")
     if not 0 <= max_tokens <= 1 << 30:
         _refuse(name, f"max_tokens must lie between 0 and 2^30, got {max_tokens}")
-    if N * M >= 1 << 31 or M * page_size >= 1 << 31:
-        _refuse(name, "the table's size and M * page_size must stay below 2^31")
-    p = (ptr(lengths), ptr(new_tokens), ptr(block_table), ptr(free_pages), ptr(free_ring))
+    if N * M >= 1 << 31 or M * page_size >= 1 << 31 or P >= 1 << 31:
+        _refuse(name, "the table's size, M * page_size and the number of pages must stay below 2^31")
+    other = _elsewhere(lengths)
+    if other is not None:
+        with other:
+            return paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_size, max_tokens)
     slots = torch.empty(max_tokens, dtype=_I64, device=dev)
     positions = torch.empty(max_tokens, dtype=_I64, device=dev)
     cu = torch.empty(N + 1, dtype=_I32, device=dev)
     granted = torch.empty(N, dtype=_I32, device=dev)
-    nws = _plan_ws(N, max_tokens)
+    nws = _plan_ws(N, M, max_tokens)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    check(lib().vm_paged_plan(p[0], p[1], p[2], ld, N, M, p[3], p[4], P, page_size, ptr(slots), ptr(positions), max_tokens, ptr(cu), ptr(granted), ptr(ws), nws,
-                              stream()), name)
+    check(lib().vm_paged_plan(lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), ld, N, M, free_pages.data_ptr(), free_ring.data_ptr(), P,
+                              page_size, slots.data_ptr(), positions.data_ptr(), max_tokens, cu.data_ptr(), granted.data_ptr(), ptr(ws), nws,
+                              stream_on(lengths.get_device())), name)
     return slots, positions, cu, granted
 
 
@@ -1329,7 +1324,6 @@ def _check_pages(name, k_pages, v_pages, other):
     return P, H, s, dh, dt
 
 
-@_on_device_of
 def paged_kv_write(k, v, k_pages, v_pages, slots):
     """Write new tokens' keys and values ``k``, ``v`` [T, Hkv, dh] (unit column stride, any other strides: column slices of a fused projection are fine)
     to ``slots`` int64 [T] of the pages; a slot outside [0, P * page_size) -- paged_plan's -1 -- writes nothing.  The slots of one call must differ
@@ -1339,18 +1333,25 @@ def paged_kv_write(k, v, k_pages, v_pages, slots):
     if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != dh or v.dtype != k.dtype or v.device != k.device:
         _refuse(name, f"k and v must be [T, {H}, {dh}] like the pages' heads, of one type, got {_desc(k)} and {_desc(v)}")
     T = k.shape[0]
+    if T >= 1 << 31 or P >= 1 << 31:
+        _refuse(name, "fewer than 2^31 tokens and pages are supported")
     ks, vs = k.stride(), v.stride()
     if ks[2] != 1 or vs[2] != 1:
         _refuse(name, f"the columns of k and v must be contiguous, got {_desc(k)} and {_desc(v)}")
     if slots.dtype != _I64 or slots.dim() != 1 or slots.shape[0] != T or (T > 1 and slots.stride(0) != 1) or slots.device != k.device:
         _refuse(name, f"slots must be a contiguous int64 tensor of the {T} tokens on their device, got {_desc(slots)}")
-    _need_inference(name, k, v, k_pages, v_pages)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        _refuse(name, "it has no backward pass: call it under torch.no_grad()")
     if T == 0:
         return
-    check(lib().vm_paged_kv_write(ptr(k), ks[0], ks[1], ptr(v), vs[0], vs[1], ptr(k_pages), ptr(v_pages), ptr(slots), T, H, dh, P, s, dt, stream()), name)
+    other = _elsewhere(k)
+    if other is not None:
+        with other:
+            return paged_kv_write(k, v, k_pages, v_pages, slots)
+    check(lib().vm_paged_kv_write(k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), T, H, dh, P, s,
+                                  dt, stream_on(k.get_device())), name)
 
 
-@_on_device_of
 def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
     """Attention of one new token per row over its paged history: ``q`` [N, Hq, dh] (unit column stride; Hq a multiple of the pages' Hkv heads: query head h
     reads key head h // (Hq / Hkv)), pages [P, Hkv, page_size, dh], ``block_table`` int32 [N, M], ``lengths`` int32 [N] (the new token's own key included,
@@ -1372,16 +1373,22 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
         _refuse(name, f"the table's rows must be contiguous and apart, got {_desc(block_table)}")
     if lengths.dtype != _I32 or lengths.dim() != 1 or lengths.shape[0] != N or (N > 1 and lengths.stride(0) != 1) or lengths.device != q.device:
         _refuse(name, f"lengths must be a contiguous int32 tensor of {N} rows on q's device, got {_desc(lengths)}")
-    if M * s >= (1 << 31) - 2048 or N * Hq >= 1 << 31:
-        _refuse(name, "M * page_size must stay below 2^31 - 2048, N * Hq below 2^31")
-    _need_inference(name, q, k_pages, v_pages)
-    o = torch.empty(N, Hq, dh, dtype=q.dtype, device=q.device)
+    if M * s >= (1 << 31) - 2048 or N * Hq >= 1 << 31 or P >= 1 << 31:
+        _refuse(name, "M * page_size must stay below 2^31 - 2048, N * Hq and the number of pages below 2^31")
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        _refuse(name, "it has no backward pass: call it under torch.no_grad()")
     if N == 0:
-        return o
+        return torch.empty_like(q)
+    other = _elsewhere(q)
+    if other is not None:
+        with other:
+            return paged_attention(q, k_pages, v_pages, block_table, lengths, scale)
+    o = torch.empty(N, Hq, dh, dtype=q.dtype, device=q.device)
     nws = _attention_ws(N, Hq, H, dh, M, s, dt)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-    check(lib().vm_paged_attention(ptr(q), qs[0], qs[1], ptr(k_pages), ptr(v_pages), ptr(block_table), ld, ptr(lengths), ptr(o), N, Hq, H, dh, P, s, M,
-                                   dh ** -0.5 if scale is None else float(scale), dt, ptr(ws), nws, stream()), name)
+    check(lib().vm_paged_attention(q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), ld, lengths.data_ptr(),
+                                   o.data_ptr(), N, Hq, H, dh, P, s, M, dh ** -0.5 if scale is None else float(scale), dt, ptr(ws), nws,
+                                   stream_on(q.get_device())), name)
     return o
 
 
@@ -1400,8 +1407,8 @@ def _token_logprobs_fwd(x, rows, targets, top, stats):
     ent = torch.empty(shape, dtype=torch.float32, device=x.device)
     best = torch.empty(shape + (top,), dtype=torch.float32, device=x.device)
     ids = torch.empty(shape + (top,), dtype=_I64, device=x.device)
-    check(lib().vm_token_logprobs_fwd(ptr(x), rows[0], rows[1], rows[2], ptr(targets), targets.numel(), V, top, ptr(logp), ptr(ent), ptr(stats), ptr(best),
-                                      ptr(ids), _DT[x.dtype], stream()), "token_logprobs")
+    check(lib().vm_token_logprobs_fwd(x.data_ptr(), rows[0], rows[1], rows[2], targets.data_ptr(), targets.numel(), V, top, logp.data_ptr(), ent.data_ptr(),
+                                      ptr(stats), best.data_ptr(), ids.data_ptr(), _DT[x.dtype], stream_on(x.get_device())), "token_logprobs")
     return logp, ent, best, ids
 
 
@@ -1417,6 +1424,7 @@ class TokenLogprobsFn(Fn):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_logp, g_ent, g_top, _g_ids):
         x, targets, stats, ent, ids = ctx.saved_tensors
         rows, V, top = ctx.rows, x.shape[-1], ids.shape[-1]
@@ -1429,7 +1437,6 @@ class TokenLogprobsFn(Fn):
         return dx[..., :V] if ld != V else dx, None, None, None
 
 
-@_on_device_of
 def token_logprobs(logits, targets, top=0):
     """Log probability of ``targets`` int64 [...] under softmax(``logits`` [..., V], float32 or bfloat16), the entropy of each distribution and its ``top``
     (<= 32) most likely columns (largest first, equal logits by ascending column), differentiable with respect to the logits through all three.
@@ -1449,6 +1456,10 @@ def token_logprobs(logits, targets, top=0):
     if targets.numel() == 0:
         z = logits.float().sum(-1)
         return TokenLogprobs(z, z.clone(), z.new_zeros(*shape, top), targets.new_zeros(*shape, top))
+    other = _elsewhere(logits)
+    if other is not None:
+        with other:
+            return token_logprobs(logits, targets, top)
     x = logits
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
