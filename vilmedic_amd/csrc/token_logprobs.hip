@@ -59,6 +59,34 @@ template <> struct LpVec<float> {
     static __device__ __forceinline__ void store(float* p, const float* f) { __builtin_nontemporal_store(lp_u4a4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])}, reinterpret_cast<lp_u4a4*>(p)); }
 };
 
+// descending sort of a wave's 64 values (bitonic; every merge starts with a mirrored step, so that all steps keep the larger value in the lower
+// lane): 21 steps of a DPP move or a row swap, a max, a min and a select
+template <int CTRL> __device__ __forceinline__ float lp_keep(float v, bool lower) { const float o = dpp_f32<CTRL>(v); return lower ? fmaxf(v, o) : fminf(v, o); }
+__device__ __forceinline__ float lp_pick(float v, float o, bool lower) { return lower ? fmaxf(v, o) : fminf(v, o); }
+__device__ __forceinline__ float lp_xor16(float v, bool lower) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(lower ? a[1] : a[0]);
+}
+__device__ __forceinline__ float lp_xor32(float v, bool lower) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(lower ? a[1] : a[0]);
+}
+__device__ __forceinline__ float lp_sort_wave(float v) {
+    const int lane = threadIdx.x & 63;
+    const bool l1 = !(lane & 1), l2 = !(lane & 2), l4 = !(lane & 4), l8 = !(lane & 8), l16 = !(lane & 16), l32 = !(lane & 32);
+    auto x4 = [&](float a) { return lp_pick(a, dpp_f32<0x1B>(dpp_f32<0x141>(a)), l4); };       // lane ^ 7, then ^ 3
+    auto tail4 = [&](float a) { return lp_keep<0xB1>(lp_keep<0x4E>(a, l2), l1); };              // lane ^ 2, ^ 1
+    v = lp_keep<0xB1>(v, l1);
+    v = lp_keep<0xB1>(lp_keep<0x1B>(v, l2), l1);                                                // ^ 3, ^ 1
+    v = tail4(lp_keep<0x141>(v, l4));                                                           // ^ 7, ^ 2, ^ 1
+    v = tail4(x4(lp_keep<0x140>(v, l8)));                                                       // ^ 15, ^ 4, ..
+    v = lp_pick(v, lp_xor16(dpp_f32<0x140>(v), l16), l16);                                      // ^ 31
+    v = tail4(x4(lp_keep<0x128>(v, l8)));                                                       // ^ 8, ^ 4, ..
+    v = lp_pick(v, lp_xor32(lp_xor16(dpp_f32<0x140>(v), l16), l32), l32);                       // ^ 63
+    v = lp_pick(v, lp_xor16(v, l16), l16);                                                      // ^ 16
+    return tail4(x4(lp_keep<0x128>(v, l8)));
+}
+
 struct LogprobArgs {
     const void* x; int64_t ld_outer, ld_inner; int inner;      // row r starts at (r / inner) * ld_outer + (r % inner) * ld_inner
     const int64_t* target; int V, top; float* logp; float* ent; float* stats; float* top_logp; int64_t* top_ids;
@@ -93,12 +121,22 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     __shared__ int s_n, s_owners;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
-    const int full = p.V / E;                                   // whole pieces; the rest is read element by element
+    // whole pieces, and single logits behind them; a row whose pieces would leave too few threads with a maximum for the alternatives' bound is read in
+    // single logits altogether (1000000 x 100 bf16, n = 16: 3.0 ms in pieces, all 100 logits candidates, against 0.77)
+    const int full = p.V / E >= min(THREADS, 2 * p.top) ? p.V / E : 0, single = p.V - full * E;
     if (tid == 0) s_n = s_owners = 0;
     LpSum a;
+    uint4 raw[LP_U];                                            // (a lone wave's row of one turn stays here for the alternatives)
+    float el[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const int c = full * E + tid + j * THREADS;
+        el[j] = -INFINITY;
+        if (j * THREADS >= single) continue;
+        if (c < p.V) el[j] = Vec::at(x + c);
+    }
     for (int c0 = 0; c0 < full; c0 += LP_U * THREADS) {
         const int ch = c0 + tid;
-        uint4 raw[LP_U];
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
             raw[u] = lp_none<T>();
@@ -120,11 +158,16 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
             for (int j = 0; j < E; ++j) a.add(f[u][j]);
         }
     }
-    const int rest = full * E + tid;                            // the last V % E logits, one thread each
-    if (rest < p.V) {
-        const float v = Vec::at(x + rest);
-        if (v > a.m) a.rise(v);
-        a.add(v);
+    {
+        float mx = -FLT_MAX;
+#pragma unroll
+        for (int j = 0; j < E; ++j) mx = fmaxf(mx, el[j]);
+        if (mx > a.m) a.rise(mx);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if (j * THREADS >= single) break;
+            a.add(el[j]);
+        }
     }
     const float mine = a.m;                                     // this thread's own maximum
     // the row's sums
@@ -137,15 +180,13 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     a.rise(m);
     const float ws = wave_sum(a.s), ww = wave_sum(a.w);
     if (lane == 0) { sh[1][wave] = ws; sh[2][wave] = ww; }
-    // (the alternatives' bound in the same round: n times the wave's largest remaining maximum)
+    // (the alternatives' bound in the same round: the wave's largest maxima in order)
     if (p.top > 0) {
-        float cur = mine, bound = -FLT_MAX;
-        for (int k = 0; k < p.top; ++k) {
-            bound = wave_max(cur);
-            if (cur == bound) cur = -FLT_MAX;
-            if (lane == 0) s_tops[wave * VM_MAX_TOP_LOGPROBS + k] = bound;
-        }
-        if (WAVES == 1 && tid == 0) s_bound = bound;
+        float sorted;
+        if (p.top == 1) sorted = wave_max(mine);
+        else sorted = lp_sort_wave(mine);
+        if (WAVES == 1) { if (lane == p.top - 1) s_bound = sorted; }
+        else if (lane < p.top) s_tops[wave * p.top + lane] = sorted;
     }
     __syncthreads();
     float s = 0.f, w = 0.f;
@@ -161,15 +202,10 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     if (p.top == 0) return;
     if (WAVES > 1) {                                            // the n-th largest of the waves' lists
         for (int i = tid; i < WAVES * p.top; i += THREADS) {
-            const int mine_at = i / p.top * VM_MAX_TOP_LOGPROBS + i % p.top;
-            const float v = s_tops[mine_at];
+            const float v = s_tops[i];
             int above = 0;
-            for (int q = 0; q < WAVES; ++q)
-                for (int k = 0; k < p.top; ++k) {
-                    const int at = q * VM_MAX_TOP_LOGPROBS + k;
-                    const float o = s_tops[at];
-                    above += o > v || (o == v && at < mine_at) ? 1 : 0;
-                }
+#pragma unroll 8
+            for (int q = 0; q < WAVES * p.top; ++q) { const float o = s_tops[q]; above += o > v || (o == v && q < i) ? 1 : 0; }
             if (above == p.top - 1) s_bound = v;
         }
         __syncthreads();
@@ -189,22 +225,36 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
         at += __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0));
         if (v >= L && at < LP_CAND) cand[at] = make_float2(v, __int_as_float(c));
     };
-    if (mine >= L) s_list[atomicAdd(&s_owners, 1)] = tid;
-    look(rest, rest < p.V ? Vec::at(x + rest) : -INFINITY);       // (every lane takes part, so that a wave's count stays one number; L > -inf)
-    __syncthreads();
-    // the owners' pieces once more, dealt out to all threads
-    const int owners = s_owners, pieces = owners * ((full + THREADS - 1) / THREADS);
-    for (int i0 = 0; i0 < pieces; i0 += THREADS) {
-        const int i = i0 + tid, turn = i / owners, ch = i < pieces ? s_list[i - turn * owners] + turn * THREADS : full;
-        uint4 raw = lp_none<T>();
-        if (ch < full) raw = Vec::load(x + (int64_t)ch * E);
+    auto look_piece = [&](int ch, const uint4 piece) {           // (every lane takes part, so that a wave's count stays one number; L > -inf)
         float f[E], mx = -INFINITY;
-        Vec::unpack(raw, f);
+        Vec::unpack(piece, f);
 #pragma unroll
         for (int j = 0; j < E; ++j) mx = fmaxf(mx, f[j]);
         if (__any(mx >= L)) {
 #pragma unroll
             for (int j = 0; j < E; ++j) look(ch * E + j, f[j]);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        if (j * THREADS >= single) break;
+        const int c = full * E + tid + j * THREADS;
+        if (WAVES > 1) el[j] = c < p.V ? Vec::at(x + c) : -INFINITY;       // (again: registers held through the pass would cost it waves)
+        look(c, el[j]);
+    }
+    if (WAVES == 1 && full <= LP_U * THREADS) {                               // the pieces are still in the registers
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            if (u * THREADS >= full) break;
+            look_piece(tid + u * THREADS, raw[u]);
+        }
+    } else {                                                    // the owners' pieces once more, dealt out to all threads
+        if (mine >= L) s_list[atomicAdd(&s_owners, 1)] = tid;
+        __syncthreads();
+        const int owners = s_owners, pieces = owners * ((full + THREADS - 1) / THREADS);
+        for (int i0 = 0; i0 < pieces; i0 += THREADS) {
+            const int i = i0 + tid, turn = i / owners, ch = i < pieces ? s_list[i - turn * owners] + turn * THREADS : full;
+            look_piece(ch, ch < full ? Vec::load(x + (int64_t)ch * E) : lp_none<T>());
         }
     }
     __syncthreads();
@@ -310,7 +360,7 @@ static int logprob_check(const void* x, int R, int inner, int V, int top, int dt
     return VM_OK;
 }
 // Threads per row, by the 16-byte pieces of a row.  Forward: one wave where a row is short and there are rows enough to fill the chip with waves (no
-// barriers, many rows in flight): 100000 x 1000 bf16 110 us with 64 threads, 195 with 128, 292 with 256; 20000 x 8832 bf16 86 / 102 / 103;
+// barriers, many rows in flight): 100000 x 1000 bf16 with 5 alternatives 96 us with 64 threads, 195 with 128, 292 with 256; 20000 x 8832 bf16 86 / 102 / 103;
 // longer rows the other way round: 10000 x 8832 fp32 82 / 76 / 71, 8192 x 30522 bf16 - / 123 / 115.  Backward (no reduction): about one batch of
 // LP_U pieces per thread: 100000 x 1000 bf16 106 us with 64 threads, 144 with 128, 176 with 256, 676 with 1024; 20000 x 8832 bf16 111 with 256, 118 with 512, 184
 // with 1024; 10000 x 8832 fp32 116 / 108 / 120; 8192 x 30522 bf16 169 / 164 / 157.
