@@ -1431,9 +1431,10 @@ class TokenLogprobsFn(Fn):
         ld = rows[1] if V <= rows[1] < V + 8 else V                   # the logits' own padded rows, where they have such
         dx = torch.empty(x.shape[:-1] + (ld,), dtype=x.dtype, device=x.device)
         g = [t.float().contiguous() if t is not None else None for t in (g_logp, g_ent, g_top if top else None)]
-        with torch.cuda.device(x.device):
-            check(lib().vm_token_logprobs_bwd(ptr(x), rows[0], rows[1], rows[2], ptr(targets), targets.numel(), V, top, ptr(stats), ptr(ent), ptr(ids), ptr(g[0]),
-                                              ptr(g[1]), ptr(g[2]), ptr(dx), ld, _DT[x.dtype], stream()), "token_logprobs")
+        with _elsewhere(x) or contextlib.nullcontext():
+            check(lib().vm_token_logprobs_bwd(x.data_ptr(), rows[0], rows[1], rows[2], targets.data_ptr(), targets.numel(), V, top, stats.data_ptr(), ent.data_ptr(),
+                                              ids.data_ptr(), ptr(g[0]), ptr(g[1]), ptr(g[2]), dx.data_ptr(), ld, _DT[x.dtype], stream_on(x.get_device())),
+                  "token_logprobs")
         return dx[..., :V] if ld != V else dx, None, None, None
 
 
