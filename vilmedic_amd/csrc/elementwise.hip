@@ -87,21 +87,22 @@ extern "C" int vm_add_bf16(const void* a, const void* b, void* out, int64_t n, v
 }
 
 // ------------------------------------------------------------------ column sum (bias gradients):  out[c] += sum_r x[r,c]
-// block = 32 column-chunks (256 columns) x 8 row lanes; grid.y splits the rows; one atomicAdd per column per block
-__global__ __launch_bounds__(256) void colsum_kernel(const bf16_t* __restrict__ x, int64_t ldx, float* __restrict__ out, int rows, int cols, const float* __restrict__ scale_dev) {
-    __shared__ float part[8][257];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int c0 = blockIdx.x * 256 + tx * 8;
+// One workgroup per 32 columns (64 bytes of every row) walks ALL rows: 4 column chunks x 256 row lanes, four 16-B loads in flight per thread, sums in a
+// fixed order (lanes, then waves).  One addition per column and launch, so equal inputs give equal bits: with the rows split over workgroups that added
+// their parts atomically, two runs of one backward pass differed in a bias gradient now and then.
+__global__ __launch_bounds__(1024) void colsum_kernel(const bf16_t* __restrict__ x, int64_t ldx, float* __restrict__ out, int rows, int cols, const float* __restrict__ scale_dev) {
+    __shared__ float part[16][33];
+    const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c0 = blockIdx.x * 32 + tx * 8;
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (c0 < cols) {
         const bool full = c0 + 8 <= cols;
-        const int step = gridDim.y * 8;
-        int r = blockIdx.y * 8 + ty;
+        int r = ty;
         if (full) {
-            for (; r + 3 * step < rows; r += 4 * step) {        // four independent 16-B loads in flight per thread
+            for (; r + 3 * 256 < rows; r += 4 * 256) {
                 uint4 v[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uint4*>(x + (int64_t)(r + u * step) * ldx + c0);
+                for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const uint4*>(x + (int64_t)(r + u * 256) * ldx + c0);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     float f[8];
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256) void colsum_kernel(const bf16_t* __restrict__ 
                 }
             }
         }
-        for (; r < rows; r += step) {
+        for (; r < rows; r += 256) {
             const bf16_t* p = x + (int64_t)r * ldx + c0;
             if (full) {
                 float f[8];
@@ -124,13 +125,18 @@ __global__ __launch_bounds__(256) void colsum_kernel(const bf16_t* __restrict__ 
         }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[ty][tx * 8 + j] = acc[j];
+    for (int j = 0; j < 8; ++j) {
+        float t = acc[j];
+#pragma unroll
+        for (int d = 4; d < 64; d <<= 1) t += __shfl_xor(t, d);            // the wave's 16 row lanes of this chunk
+        if (lane < 4) part[wave][tx * 8 + j] = t;
+    }
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c < cols) {
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && c < cols) {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t += part[k][threadIdx.x];
+        for (int k = 0; k < 16; ++k) t += part[k][threadIdx.x];
         atomicAdd(out + c, scale_dev ? t * (*scale_dev) : t);
     }
 }
@@ -138,8 +144,7 @@ extern "C" int vm_colsum_bf16(const void* x, int64_t ldx, float* out, int rows, 
     VM_REQUIRE(x && out && rows > 0 && cols > 0 && (ldx % 8) == 0, "vm_colsum_bf16: bad arguments");
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_ELT, 2.0 * rows * (double)cols, s);
-    int gy = (rows + 63) / 64; if (gy > 128) gy = 128; if (gy < 1) gy = 1;
-    hipLaunchKernelGGL(colsum_kernel, dim3((cols + 255) / 256, gy), dim3(256), 0, s, (const bf16_t*)x, ldx, out, rows, cols, scale_dev);
+    hipLaunchKernelGGL(colsum_kernel, dim3((cols + 31) / 32), dim3(1024), 0, s, (const bf16_t*)x, ldx, out, rows, cols, scale_dev);
     return vm_check_launch("vm_colsum_bf16");
 }
 
