@@ -123,6 +123,50 @@ def test_plan_clamps_lengths_and_marks_pages_that_do_not_exist():
     assert lengths.tolist() == [1, 32, 21, 18] and table[0].tolist() == [6, -1] and ring.tolist() == [0, 0]
 
 
+def test_plan_counts_far_beyond_everything_without_overflow():
+    from vilmedic_amd import ops
+    big = 2 ** 31 - 1
+    o = PlanOracle(5, 4, 16, list(range(20)))
+    new = [3, big, big, 5, big]
+    lengths, table = torch.zeros(5, dtype=I32, device=dev()), torch.full((5, 4), -1, dtype=I32, device=dev())
+    free, ring = torch.arange(20, dtype=I32, device=dev()), torch.tensor([0, 20], dtype=I32, device=dev())
+    got = ops.paged_plan(lengths, torch.tensor(new, dtype=I32, device=dev()), table, free, ring, 16, 64)
+    want = o.plan(new, 64)
+    assert got[3].tolist() == want[3] == [3, 0, 0, 0, 0]                               # row 3's tokens lie behind max_tokens in the packed order
+    for a, b in zip(got, want):
+        assert a.tolist() == b
+    same_state(o, lengths, table, free, ring)
+    many = torch.full((3000,), big, dtype=I32, device=dev())
+    lengths, table = torch.zeros(3000, dtype=I32, device=dev()), torch.full((3000, 1), -1, dtype=I32, device=dev())
+    slots, _, cu, granted = ops.paged_plan(lengths, many, table, free, ring, 16, 7)
+    assert not granted.any() and not lengths.any() and bool((slots == -1).all()) and cu.tolist() == [0] + [7] * 3000
+
+
+@pytest.mark.parametrize("N,M", [(40, 8), (1500, 3)])
+def test_plan_replayed_from_a_graph(N, M):
+    """one launch, and two launches with scratch memory: every replay takes the step after the last one"""
+    from vilmedic_amd import ops
+    P = N * M
+    o = PlanOracle(N, M, 16, list(range(P)))
+    lengths, table = torch.zeros(N, dtype=I32, device=dev()), torch.full((N, M), -1, dtype=I32, device=dev())
+    free, ring = torch.arange(P, dtype=I32, device=dev()), torch.tensor([0, P], dtype=I32, device=dev())
+    new = torch.zeros(N, dtype=I32, device=dev())
+    graph = torch.cuda.CUDAGraph()
+    with ops.capture(graph):
+        out = ops.paged_plan(lengths, new, table, free, ring, 16, 3 * N)
+    g = torch.Generator().manual_seed(N)
+    for step in range(8):
+        n = torch.randint(-1, 4, (N,), generator=g)
+        new.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, o.plan(n.tolist(), 3 * N)):
+            assert a.tolist() == b, step
+        same_state(o, lengths, table, free, ring)
+        ops.paged_plan(lengths, torch.zeros_like(new), table, free, ring, 16, 0)      # an eager plan in between: nothing to do
+        o.plan([0] * N, 0)
+
+
 # ----------------------------------------------------------------------------- write
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("T,H,dh,s,skew", [(1, 1, 8, 16, 0), (5, 2, 40, 16, 0), (64, 12, 64, 16, 8), (33, 3, 96, 32, 1), (700, 8, 128, 64, 0), (9, 1, 256, 128, 3), (257, 2, 48, 16, 4)])
@@ -217,7 +261,8 @@ def check_attention(q, k, v, table, lengths, scale=None, got=None):
 SHAPES = [  # N, Hq, H, dh, page, lengths
     (1, 1, 1, 8, 16, [1]), (2, 1, 1, 64, 16, [0, 5]), (4, 12, 12, 64, 16, [1, 15, 16, 17]), (5, 8, 2, 128, 16, [31, 32, 33, 63, 65]),
     (3, 16, 1, 64, 16, [128, 129, 200]), (2, 20, 1, 32, 32, [77, 300]), (2, 32, 1, 128, 16, [100, 1]), (3, 6, 2, 48, 16, [0, 47, 511]), (2, 10, 2, 96, 64, [640, 1000]),
-    (2, 4, 4, 40, 16, [90, 91]), (2, 6, 3, 80, 32, [256, 257]), (3, 4, 1, 256, 16, [5, 64, 700]), (2, 2, 1, 160, 128, [129, 1]), (1, 8, 8, 128, 256, [3000]), (2, 7, 1, 72, 16, [1025, 4])]
+    (2, 4, 4, 40, 16, [90, 91]), (2, 6, 3, 80, 32, [256, 257]), (3, 4, 1, 256, 16, [5, 64, 700]), (2, 2, 1, 160, 128, [129, 1]), (1, 8, 8, 128, 256, [3000]), (2, 7, 1, 72, 16, [1025, 4]), (2, 16, 1, 256, 16, [33, 400]), (1, 33, 1, 256, 32, [90]),
+    (2, 4, 2, 64, 4096, [4097, 5000])]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])

@@ -23,19 +23,18 @@ def reference(x, t, top, g=None):
     x = x.double()
     R, V = x.shape
     m = x.amax(1, keepdim=True)
-    z = torch.logsumexp(x, 1, keepdim=True)
-    lp = x - z
+    ls = torch.log((x - m).exp().sum(1))                 # (kept apart from m: next to 3e38 even 64 bits lose it)
+    lp = (x - m) - ls[:, None]
     p = lp.exp()
     d = torch.where(p > 0, x - m, torch.zeros_like(x))
     Ed, Ed2 = (p * d.abs()).sum(1), (p * d * d).sum(1)
-    ls = (z - m)[:, 0]
     ent = -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(1)
     e_ls = (V / 64 + 38 + 2 * Ed) * U
     e_ent = (V / 64 + 44 + 4 * Ed) * U * (1 + Ed + ls.abs()) + 2 * U * Ed2
     ok = (t >= 0) & (t < V)
     tt = t.clamp(0, V - 1)
     xt = x.gather(1, tt[:, None])[:, 0]
-    logp = torch.where(ok, xt - z[:, 0], torch.where(t < 0, torch.zeros_like(xt), torch.full_like(xt, float("nan"))))
+    logp = torch.where(ok, (xt - m[:, 0]) - ls, torch.where(t < 0, torch.zeros_like(xt), torch.full_like(xt, float("nan"))))
     e_logp = e_ls + 4 * U * ((xt - m[:, 0]).abs().nan_to_num(posinf=0) + ls.abs())
     ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :top]
     best = lp.gather(1, ids)
@@ -156,6 +155,21 @@ def test_banned_columns_and_empty_rows(dtype, V):
     assert out.logp[5].item() == -inf and torch.isfinite(out.entropy[5])
     grad = torch.autograd.grad(out.entropy.sum() + out.top_logp[:, 0].sum(), xd)[0]
     assert bool(torch.isfinite(grad).all()) and not bool(grad[3].any()) and not bool(grad[torch.isinf(xd)].any())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [30, 700, 40000])
+def test_the_lowest_value_of_the_type_is_a_logit_like_any_other(dtype, V):
+    """rows masked with finfo.min instead of -inf: uniform where nothing else is left, without weight next to ordinary logits"""
+    x, _, _ = make(4, V, dtype, seed=5)
+    low = torch.finfo(dtype).min
+    x[0] = low
+    x[1, ::2] = low
+    x[2, 1:] = low
+    x[3, :7] = low
+    x[3, 7:] = -float("inf")
+    g = (torch.tensor([1.0, -2.0, 0.5, 1.5]), torch.tensor([0.3, 0.2, -1.0, 0.7]))
+    check(x, torch.tensor([3, 1, 0, 2]), 5, g=g)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])

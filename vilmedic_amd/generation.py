@@ -128,7 +128,7 @@ class DecodeState:
             self.paged = PagedKVCache(len(self.layers), self.M, self.H, self.dhp, self.T, page_size=paged[0], pages=paged[1], dtype=self.act, device=dev)
             self.buf_kv = torch.empty(self.M, 2 * self.Da, dtype=self.act, device=dev)        # K|V of the new tokens, one row each
             self.slots = torch.empty(self.M, dtype=torch.long, device=dev)
-            self.alive = None                 # uint8 / bool [M]: rows that still decode (None: all of them); set by the driver
+            self.alive = None                 # uint8 / bool [M]: rows that still decode (None: all of them); set by the decode loop
             self.starved = torch.zeros(self.M, dtype=torch.bool, device=dev)
         self.self_kv = [None if paged is not None else torch.empty(self.M * self.T, 2 * self.Da, dtype=self.act, device=dev) for _ in self.layers]
         self.pw = None                    # per layer: the padded weights / biases of a padded-head step (built by load_encoder)
