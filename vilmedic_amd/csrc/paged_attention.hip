@@ -26,6 +26,7 @@
 #include "common.h"
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t pa_u3 __attribute__((ext_vector_type(3), aligned(4)));
 // 16 bytes of the cache, read once in this call and marked as such (a step's other data keeps its place in the caches; 153 -> 148 us for 0.8 GB)
 __device__ __forceinline__ uint4_t pa_ld(const void* p) { return __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)); }
 
@@ -50,11 +51,11 @@ __device__ __forceinline__ float pa_col_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// W columns of V per lane (16 W >= dh), SUB 16-key subtiles per tile
-template <typename T, int W> struct PaTile;
+// DK columns of K and Q (a multiple of 32), W columns of V per lane (16 W >= dh; a multiple of W, or of 8 where W is 16, is where a head may end), SUB 16-key subtiles per tile
+template <typename T, int W, int DK> struct PaTile;
 
-template <int W> struct PaTile<bf16_t, W> {
-    static constexpr int SUB = 2, KC = (16 * W + 31) / 32;       // K fragments of 32 columns: 8 per lane
+template <int W, int DK> struct PaTile<bf16_t, W, DK> {
+    static constexpr int SUB = 2, KC = DK / 32;                  // K fragments of 32 columns: 8 per lane
     static constexpr int VD = W / 2;                              // dwords of V per lane and key
     struct Q { uint4 q[KC]; };
     uint4 k[SUB][KC];
@@ -90,6 +91,7 @@ template <int W> struct PaTile<bf16_t, W> {
         for (int i = 0; i < 4; ++i) {
             const bf16_t* p = base + (g * 4 + i) * dh;
             if constexpr (VD == 1) v[u][i][0] = *reinterpret_cast<const uint32_t*>(p + min(r * W, dh - W));
+            else if constexpr (VD == 3) { const pa_u3 x = *reinterpret_cast<const pa_u3*>(p + min(r * W, dh - W)); v[u][i][0] = x[0]; v[u][i][1] = x[1]; v[u][i][2] = x[2]; }
             else if constexpr (VD == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p + min(r * W, dh - W)); v[u][i][0] = x.x; v[u][i][1] = x.y; }
             else {
 #pragma unroll
@@ -147,8 +149,8 @@ template <int W> struct PaTile<bf16_t, W> {
 };
 
 // fp32: exact products on the f32 matrix instruction (4 columns / 4 keys per step; element j of a lane's 16 B feeds step j)
-template <int W> struct PaTile<float, W> {
-    static constexpr int SUB = 1, KC = W;
+template <int W, int DK> struct PaTile<float, W, DK> {
+    static constexpr int SUB = 1, KC = DK / 16;
     struct Q { float4_t q[KC]; };
     float4_t k[SUB][KC];
     float v[SUB][4][W];
@@ -174,8 +176,10 @@ template <int W> struct PaTile<float, W> {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float* p = base + (g * 4 + i) * dh;
-            if constexpr (W == 2) { const float2 x = *reinterpret_cast<const float2*>(p + min(r * W, dh - W)); v[u][i][0] = x.x; v[u][i][1] = x.y; }
-            else {
+            if constexpr (W == 2 || W == 6) {
+#pragma unroll
+                for (int d = 0; d < W; d += 2) { const float2 x = *reinterpret_cast<const float2*>(p + min(r * W + d, dh - 2)); v[u][i][d] = x.x; v[u][i][d + 1] = x.y; }
+            } else {
 #pragma unroll
                 for (int d = 0; d < W; d += 4) {
                     const float4_t x = __builtin_bit_cast(float4_t, pa_ld(p + min(r * W + d, dh - 4)));
@@ -214,12 +218,12 @@ __device__ __forceinline__ void pa_range(int tiles, int parts, int w, int& t0, i
     t0 = min(w * per, tiles);
     t1 = min(t0 + per, tiles);
 }
-template <typename T, int W> __host__ __device__ constexpr int pa_tile_keys() { return 16 * PaTile<T, W>::SUB; }
+template <typename T> constexpr int pa_tile_keys() { return 16 * PaTile<T, 2, 32>::SUB; }
 
-template <typename T, int W, int WAVES>
+template <typename T, int W, int DK, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_kernel(const PagedAttnArgs p) {
     extern __shared__ __attribute__((aligned(16))) float pa_sm[];      // [waves][16][2] (m, l) | [waves][queries][dh] O
-    constexpr int SUB = PaTile<T, W>::SUB, TK = 16 * SUB;
+    constexpr int SUB = PaTile<T, W, DK>::SUB, TK = 16 * SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     int b = blockIdx.x;
     const int split = b % p.splits; b /= p.splits;
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
         if (key < limit) { const int page = row[key >> p.shift]; pages = page >= 0 && page < p.P ? page : -1; }
     };
     if (first == 0) fetch(cap);
-    using Tile = PaTile<T, W>;
+    using Tile = PaTile<T, W, DK>;
     typename Tile::Q q;
     Tile::load_q(q, (const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, p.dh, r < nq, p.q_wide);
     const int len = min(max(p.lengths[n], 0), cap), tiles = (len + TK - 1) / TK;
@@ -410,11 +414,12 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
 
 // How many workgroups share a row's keys.  The chip's 256 CUs are fed evenly by 256, 512, ... workgroups: one 40001-token row with 8 key heads took 33 us on
 // 160 workgroups, 38 on 320 (64 CUs have twice the work of the others) and 40 on 632.  So: as many rounds of 256 (up to 8) as leave a workgroup
-// 1024 keys of a full row (fewer keys where the rows are short and few: at least 256), shared by the rows.
+// 1024 keys of a full row (fewer keys where the rows are short and few: at least 256), shared by the rows; several rows are rarely all full, they get 512 (16
+// rows up to 18000 with 2 key heads 42 -> 38 us, 2 rows up to 20000 with 12 41 -> 36, 48 rows up to 8192 with 8 the same; 256 keys lose again).
 static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
     const int64_t blocks = (int64_t)N * Hkv * ((Hq / Hkv + 15) / 16);
     const int64_t keys = (int64_t)M * page_size, most = (keys + 255) / 256;
-    int64_t rounds = keys * blocks / (256 * 1024);
+    int64_t rounds = keys * blocks / (256 * (N > 1 ? 512 : 1024));
     rounds = rounds < 1 ? 1 : (rounds > 8 ? 8 : rounds);
     int64_t s = 256 * rounds / blocks;
     if (s > most) s = most;
@@ -428,28 +433,30 @@ extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, i
     return s == 1 ? 0 : (size_t)N * Hq * s * (dh + 2) * sizeof(float);
 }
 
-template <typename T, int W, int WAVES>
+template <typename T, int W, int DK, int WAVES>
 static void pa_launch_waves(const PagedAttnArgs& a, hipStream_t s) {
     const int nq = a.G < 16 ? a.G : 16;
     const size_t lds = sizeof(float) * (WAVES * 32 + (size_t)WAVES * nq * a.dh);
-    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL((paged_attention_kernel<T, W, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
+    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, DK, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((paged_attention_kernel<T, W, DK, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
 }
 // One wave per row and head, without the merge of four, where that alone fills the chip (12 waves for each of its 256 CUs): 256 rows x 12 heads of up to 128
 // fp32 keys 27.8 us against 30.0; 64 rows the other way round, 9.6 us against 7.6.
 #define PA_ONE (256 * 12)
-template <typename T, int W>
+template <typename T, int W, int DK>
 static void pa_launch(const PagedAttnArgs& a, hipStream_t s) {
-    if (a.splits == 1 && (int64_t)a.N * a.Hk * a.qblocks >= PA_ONE) return pa_launch_waves<T, W, 1>(a, s);
-    pa_launch_waves<T, W, PA_WAVES>(a, s);
-    if (a.splits > 1) hipLaunchKernelGGL(paged_attention_join_kernel<T>, dim3(a.N * a.Hq), dim3(256), 0, s, a, pa_tile_keys<T, W>());
+    if (a.splits == 1 && (int64_t)a.N * a.Hk * a.qblocks >= PA_ONE) return pa_launch_waves<T, W, DK, 1>(a, s);
+    pa_launch_waves<T, W, DK, PA_WAVES>(a, s);
+    if (a.splits > 1) hipLaunchKernelGGL(paged_attention_join_kernel<T>, dim3(a.N * a.Hq), dim3(256), 0, s, a, pa_tile_keys<T>());
 }
 template <typename T>
 static void pa_launch_w(const PagedAttnArgs& a, hipStream_t s) {
-    if (a.dh <= 32) pa_launch<T, 2>(a, s);
-    else if (a.dh <= 64) pa_launch<T, 4>(a, s);
-    else if (a.dh <= 128) pa_launch<T, 8>(a, s);
-    else pa_launch<T, 16>(a, s);
+    if (a.dh <= 32) pa_launch<T, 2, 32>(a, s);
+    else if (a.dh <= 64) pa_launch<T, 4, 64>(a, s);
+    else if (a.dh <= 96 && a.dh % 6 == 0) pa_launch<T, 6, 96>(a, s);      // 72 and 96: no lane's columns may straddle the head's end
+    else if (a.dh <= 96) pa_launch<T, 8, 96>(a, s);
+    else if (a.dh <= 128) pa_launch<T, 8, 128>(a, s);
+    else pa_launch<T, 16, 256>(a, s);
 }
 
 extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages,
