@@ -109,3 +109,26 @@ def test_sampled_tokens_have_their_logprobs_too(golden):
                        generator=torch.Generator().manual_seed(3), **kw)
     assert out.logprobs.logp.shape == (g["B"], out.sequences.shape[1] - 1) and bool((out.logprobs.logp <= 0).all()) and bool(torch.isfinite(out.logprobs.entropy).all())
     assert out.logprobs.top_ids.shape[-1] == 0 and bool((out.logprobs.logp[:, 0] < 0).all())
+
+
+def test_the_step_by_step_loop_on_pages(golden):
+    g, cfg, dec, kw = setup(golden)
+    ref = g["beams1_lp1.0"]["sequences"]
+    out = dec.generate(kv_cache="paged", output_scores=True, output_logprobs=1, return_dict_in_generate=True, **kw)
+    assert torch.equal(out.sequences.cpu(), ref) and len(out.scores) == ref.shape[1] - 1 and out.logprobs.logp.shape[1] == ref.shape[1] - 1
+    need = peak_pages(ref, 2, 16)
+    assert torch.equal(dec.generate(kv_cache="paged", kv_pages=need, output_scores=True, return_dict_in_generate=True, **kw).sequences.cpu(), ref)
+
+
+def test_logprobs_of_an_ensemble_are_those_of_the_summed_logits(golden):
+    g, cfg, dec, kw = setup(golden)
+    eo = dict(encoder_hidden_states=kw.pop("encoder_hidden_states"), encoder_attention_mask=kw.pop("encoder_attention_mask"))
+    call = dict(hf_models=[dec.decoder, dec.decoder], encoders_outputs=[eo, eo], return_dict_in_generate=True, **kw)
+    ref = dec.generate(output_scores=True, **call)
+    kept = torch.log_softmax(torch.stack([s.clone() for s in ref.scores], 1).double(), -1)
+    out = dec.generate(output_logprobs=0, **call)
+    assert torch.equal(out.sequences, ref.sequences)
+    want = kept.gather(2, out.sequences[:, 1:, None])[..., 0]
+    is_eos = (out.sequences[:, 1:] == 2).long()
+    live = (torch.cumsum(is_eos, 1) - is_eos) == 0
+    assert float((out.logprobs.logp.double() - want)[live].abs().max()) <= 1e-4 and not bool(out.logprobs.logp[~live].any())
