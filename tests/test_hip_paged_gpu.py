@@ -357,6 +357,21 @@ def test_attention_propagates_nan_and_inf_of_live_keys_only(dtype):
     assert bool((got[2, :, 7] == float("inf")).all()) and bool(torch.isfinite(got[2, :, :7]).all()) and bool(torch.isfinite(got[2, :, 8:]).all())
 
 
+@pytest.mark.parametrize("dh", [8, 40, 64, 72, 80, 96, 104, 160, 256])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_gives_a_key_of_score_minus_infinity_no_weight(dtype, dh):
+    """an infinity in a key's last column, against a negative query column: the row is what it is without that key (exactly zero weight)"""
+    lens = [1 + 20, 1 + 47, 1 + 700]
+    k, v, table, lengths = make_cache(dtype, 2, dh, 16, lens, seed=dh)
+    for n, length in enumerate(lens):
+        k[table[n, (length - 1) // 16], :, (length - 1) % 16, -1] = float("inf")
+    q = torch.randn(3, 6, dh, generator=torch.Generator().manual_seed(dh)).to(dtype)
+    q[:, :, -1] = -q[:, :, -1].abs() - 0.5
+    from vilmedic_amd import ops
+    got = ops.paged_attention(*(t.to(dev()) for t in (q, k, v, table, lengths)))
+    check_attention(q, k, v, table, lengths - 1, got=got)
+
+
 def test_attention_reaches_beyond_32_bit_offsets():
     """a pool of 2.2e9 elements (4.5 GB each for K and V): pages at its very end"""
     from vilmedic_amd import ops

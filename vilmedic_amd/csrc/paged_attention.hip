@@ -20,7 +20,7 @@
 //     (a load in a branch makes the compiler wait for everything in flight).  Worth 6 % at 128 columns.
 //   * long rows are split over workgroups (``splits``); partial (m, l, O) in fp32 go to a workspace and a second launch joins them.  Each row is
 //     split by its OWN length, so the table's width decides only how many workgroups start.
-// Measured: 48 rows of 0 .. 8192 keys, 32 query and 8 key heads of 128 bf16 columns (810 MB of cache): 150 us with the join, 5.4 TB/s (a large copy: 5.2);
+// Measured: 48 rows of 0 .. 8192 keys, 32 query and 8 key heads of 128 bf16 columns (810 MB of cache): 150 - 153 us with the join, 5.3 TB/s (a large copy: 5.2);
 // one row of 40001 keys, the same heads: 32 us, 5.1 TB/s; 256 rows of up to 128 keys, 12 heads of 64 fp32 columns: 25 us, 4.2 TB/s (short rows: a
 // wave's few tiles do not cover the latency of its first); 64 rows of them in bf16: 7.4 us, three dependent trips to memory and a merge.
 #include "common.h"
@@ -101,6 +101,16 @@ template <int W, int DK> struct PaTile<bf16_t, W, DK> {
                 }
             }
         }
+    }
+    // ... and zeroed before they meet that zero: an infinity among the head's last columns would make it NaN
+    __device__ __forceinline__ void trim_k(int g, int dh) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const bool in = c * 32 + g * 8 < dh;
+                k[u][c] = make_uint4(in ? k[u][c].x : 0u, in ? k[u][c].y : 0u, in ? k[u][c].z : 0u, in ? k[u][c].w : 0u);
+            }
     }
     __device__ __forceinline__ void drop_v(int u, int i, bool ok) {
 #pragma unroll
@@ -188,6 +198,14 @@ template <int W, int DK> struct PaTile<float, W, DK> {
             }
         }
     }
+    __device__ __forceinline__ void trim_k(int g, int dh) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) k[u][c][i] = c * 16 + g * 4 < dh ? k[u][c][i] : 0.f;
+    }
     __device__ __forceinline__ void drop_v(int u, int i, bool ok) {
 #pragma unroll
         for (int d = 0; d < W; ++d) v[u][i][d] = ok ? v[u][i][d] : 0.f;
@@ -272,6 +290,7 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
 #pragma unroll
         for (int u = 0; u < SUB; ++u) whole = whole && good[u];
         float4_t s[SUB];
+        if (p.dh != DK) x.trim_k(g, p.dh);
         x.scores(q, s);
         float mx = m;
 #pragma unroll
