@@ -13,7 +13,7 @@
 //     of the bandwidth.
 //   * K goes straight from memory into the matrix unit's registers (16 B a lane, no LDS): the order in which the contraction visits the columns is
 //     free as long as Q uses the same.  V is needed with the keys along the contraction, 8 (bf16) or 4 (fp32) keys per lane; its rows are loaded
-//     as they lie, W consecutive columns a lane, and a pair of keys is interleaved with one byte permute (bf16; fp32 needs none).
+//     as they lie, consecutive columns a lane, and a pair of keys is interleaved with one byte permute (bf16; fp32 needs none).
 //   * the head's run inside a page is contiguous and a 16-key subtile never leaves its page, so a subtile's address is one scalar base (its page
 //     number, fetched 64 subtiles ahead into a register) plus offsets that no lane ever recomputes.
 //   * two tiles per wave in registers: the next one is requested before the current one is used, and nothing in the walk is loaded behind a condition
@@ -57,6 +57,7 @@ template <typename T, int W, int DK> struct PaTile;
 template <int W, int DK> struct PaTile<bf16_t, W, DK> {
     static constexpr int SUB = 2, KC = DK / 32;                  // K fragments of 32 columns: 8 per lane
     static constexpr int VD = W / 2;                              // dwords of V per lane and key
+    static constexpr int VC = W < 8 ? W : 8;                      // columns of V per load: a wave's 16 lanes lie side by side in it
     struct Q { uint4 q[KC]; };
     uint4 k[SUB][KC];
     uint32_t v[SUB][4][VD];
@@ -96,7 +97,7 @@ template <int W, int DK> struct PaTile<bf16_t, W, DK> {
             else {
 #pragma unroll
                 for (int d = 0; d < VD; d += 4) {
-                    const uint4_t x = pa_ld(p + min(r * W + 2 * d, dh - 8));
+                    const uint4_t x = pa_ld(p + min(32 * d + r * 8, dh - 8));
                     v[u][i][d] = x.x; v[u][i][d + 1] = x.y; v[u][i][d + 2] = x.z; v[u][i][d + 3] = x.w;
                 }
             }
@@ -161,6 +162,7 @@ template <int W, int DK> struct PaTile<bf16_t, W, DK> {
 // fp32: exact products on the f32 matrix instruction (4 columns / 4 keys per step; element j of a lane's 16 B feeds step j)
 template <int W, int DK> struct PaTile<float, W, DK> {
     static constexpr int SUB = 1, KC = DK / 16;
+    static constexpr int VC = W % 4 ? 2 : 4;
     struct Q { float4_t q[KC]; };
     float4_t k[SUB][KC];
     float v[SUB][4][W];
@@ -188,11 +190,11 @@ template <int W, int DK> struct PaTile<float, W, DK> {
             const float* p = base + (g * 4 + i) * dh;
             if constexpr (W == 2 || W == 6) {
 #pragma unroll
-                for (int d = 0; d < W; d += 2) { const float2 x = *reinterpret_cast<const float2*>(p + min(r * W + d, dh - 2)); v[u][i][d] = x.x; v[u][i][d + 1] = x.y; }
+                for (int d = 0; d < W; d += 2) { const float2 x = *reinterpret_cast<const float2*>(p + min(16 * d + r * 2, dh - 2)); v[u][i][d] = x.x; v[u][i][d + 1] = x.y; }
             } else {
 #pragma unroll
                 for (int d = 0; d < W; d += 4) {
-                    const float4_t x = __builtin_bit_cast(float4_t, pa_ld(p + min(r * W + d, dh - 4)));
+                    const float4_t x = __builtin_bit_cast(float4_t, pa_ld(p + min(16 * d + r * 4, dh - 4)));
                     v[u][i][d] = x[0]; v[u][i][d + 1] = x[1]; v[u][i][d + 2] = x[2]; v[u][i][d + 3] = x[3];
                 }
             }
@@ -238,8 +240,9 @@ __device__ __forceinline__ void pa_range(int tiles, int parts, int w, int& t0, i
 }
 template <typename T> constexpr int pa_tile_keys() { return 16 * PaTile<T, 2, 32>::SUB; }
 
-template <typename T, int W, int DK, int WAVES>
+template <typename T, int W, int DK, bool WHOLE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_kernel(const PagedAttnArgs p) {
+    const int dh = WHOLE ? DK : p.dh;
     extern __shared__ __attribute__((aligned(16))) float pa_sm[];      // [waves][16][2] (m, l) | [waves][queries][dh] O
     constexpr int SUB = PaTile<T, W, DK>::SUB, TK = 16 * SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
     if (first == 0) fetch(cap);
     using Tile = PaTile<T, W, DK>;
     typename Tile::Q q;
-    Tile::load_q(q, (const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, p.dh, r < nq, p.q_wide);
+    Tile::load_q(q, (const T*)p.q + n * p.q_row + (h0 + min(r, nq - 1)) * p.q_head, g, dh, r < nq, p.q_wide);
     const int len = min(max(p.lengths[n], 0), cap), tiles = (len + TK - 1) / TK;
     const bool only = p.splits == 1;
     int t0, t1;
@@ -280,9 +283,9 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
         for (int u = 0; u < SUB; ++u) {
             const int key = t * TK + u * 16, page = __builtin_amdgcn_readlane(pages, (t * SUB - first + u) & 63);
             good[u] = key < len && page >= 0;
-            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + (key & mask)) * p.dh;
-            x.load_k(u, (const T*)p.k + at, r, g, p.dh);
-            x.load_v(u, (const T*)p.v + at, r, g, p.dh);
+            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + (key & mask)) * dh;
+            x.load_k(u, (const T*)p.k + at, r, g, dh);
+            x.load_v(u, (const T*)p.v + at, r, g, dh);
         }
     };
     auto use = [&](Tile& x, const bool (&good)[SUB], int t) {
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
 #pragma unroll
         for (int u = 0; u < SUB; ++u) whole = whole && good[u];
         float4_t s[SUB];
-        if (p.dh != DK) x.trim_k(g, p.dh);
+        if (!WHOLE) x.trim_k(g, dh);
         x.scores(q, s);
         float mx = m;
 #pragma unroll
@@ -353,20 +356,20 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
     }
     l = pa_col_sum(l);
     float* ml = pa_sm + wave * 32;
-    float* so = pa_sm + WAVES * 32 + wave * nq * p.dh;
+    float* so = pa_sm + WAVES * 32 + wave * nq * dh;
     if (g == 0) { ml[2 * r] = m; ml[2 * r + 1] = l; }
     if (r < nq) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int d = 0; d < W; ++d) {
-                const int c = (g * 4 + i) * W + d;
-                if (c < p.dh) so[r * p.dh + c] = o[d][i];
+                const int c = (d / Tile::VC * 16 + g * 4 + i) * Tile::VC + d % Tile::VC;
+                if (c < dh) so[r * dh + c] = o[d][i];
             }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < nq * p.dh; e += 64 * WAVES) {
-        const int qi = e / p.dh, c = e - qi * p.dh;
+    for (int e = threadIdx.x; e < nq * dh; e += 64 * WAVES) {
+        const int qi = e / dh, c = e - qi * dh;
         float mm = -INFINITY;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, pa_sm[w * 32 + 2 * qi]);
@@ -375,14 +378,14 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             const float f = __builtin_amdgcn_exp2f(pa_sm[w * 32 + 2 * qi] - base);
-            acc = fmaf(f, pa_sm[WAVES * 32 + (w * nq + qi) * p.dh + c], acc);
+            acc = fmaf(f, pa_sm[WAVES * 32 + (w * nq + qi) * dh + c], acc);
             sum = fmaf(f, pa_sm[w * 32 + 2 * qi + 1], sum);
         }
         const int64_t out = (int64_t)n * p.Hq + h0 + qi;
         if (only) {
-            pa_store((T*)p.o + out * p.dh + c, sum == 0.f ? 0.f : acc / sum);
+            pa_store((T*)p.o + out * dh + c, sum == 0.f ? 0.f : acc / sum);
         } else {
-            p.part_o[(out * p.splits + split) * p.dh + c] = acc;
+            p.part_o[(out * p.splits + split) * dh + c] = acc;
             if (c == 0) { p.part_ml[2 * (out * p.splits + split)] = mm; p.part_ml[2 * (out * p.splits + split) + 1] = sum; }
         }
     }
@@ -452,30 +455,37 @@ extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, i
     return s == 1 ? 0 : (size_t)N * Hq * s * (dh + 2) * sizeof(float);
 }
 
-template <typename T, int W, int DK, int WAVES>
+template <typename T, int W, int DK, bool WHOLE, int WAVES>
 static void pa_launch_waves(const PagedAttnArgs& a, hipStream_t s) {
     const int nq = a.G < 16 ? a.G : 16;
     const size_t lds = sizeof(float) * (WAVES * 32 + (size_t)WAVES * nq * a.dh);
-    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, DK, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL((paged_attention_kernel<T, W, DK, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
+    if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, DK, WHOLE, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((paged_attention_kernel<T, W, DK, WHOLE, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
 }
 // One wave per row and head, without the merge of four, where that alone fills the chip (12 waves for each of its 256 CUs): 256 rows x 12 heads of up to 128
 // fp32 keys 27.8 us against 30.0; 64 rows the other way round, 9.6 us against 7.6.
 #define PA_ONE (256 * 12)
-template <typename T, int W, int DK>
+template <typename T, int W, int DK, bool WHOLE>
 static void pa_launch(const PagedAttnArgs& a, hipStream_t s) {
-    if (a.splits == 1 && (int64_t)a.N * a.Hk * a.qblocks >= PA_ONE) return pa_launch_waves<T, W, DK, 1>(a, s);
-    pa_launch_waves<T, W, DK, PA_WAVES>(a, s);
+    if (a.splits == 1 && (int64_t)a.N * a.Hk * a.qblocks >= PA_ONE) return pa_launch_waves<T, W, DK, WHOLE, 1>(a, s);
+    pa_launch_waves<T, W, DK, WHOLE, PA_WAVES>(a, s);
     if (a.splits > 1) hipLaunchKernelGGL(paged_attention_join_kernel<T>, dim3(a.N * a.Hq), dim3(256), 0, s, a, pa_tile_keys<T>());
 }
 template <typename T>
 static void pa_launch_w(const PagedAttnArgs& a, hipStream_t s) {
-    if (a.dh <= 32) pa_launch<T, 2, 32>(a, s);
-    else if (a.dh <= 64) pa_launch<T, 4, 64>(a, s);
-    else if (a.dh <= 96 && a.dh % 6 == 0) pa_launch<T, 6, 96>(a, s);      // 72 and 96: no lane's columns may straddle the head's end
-    else if (a.dh <= 96) pa_launch<T, 8, 96>(a, s);
-    else if (a.dh <= 128) pa_launch<T, 8, 128>(a, s);
-    else pa_launch<T, 16, 256>(a, s);
+    if (a.dh == 32) pa_launch<T, 2, 32, true>(a, s);
+    else if (a.dh < 32) pa_launch<T, 2, 32, false>(a, s);
+    else if (a.dh == 64) pa_launch<T, 4, 64, true>(a, s);
+    else if (a.dh < 64) pa_launch<T, 4, 64, false>(a, s);
+    else if (a.dh == 96) pa_launch<T, 6, 96, true>(a, s);
+    else if (a.dh < 96) {
+        if constexpr (sizeof(T) == 2)
+            if (a.dh % 6) return pa_launch<T, 8, 96, false>(a, s);        // 80, 88: a bf16 load of 6 columns would straddle the head's end
+        pa_launch<T, 6, 96, false>(a, s);
+    } else if (a.dh == 128) pa_launch<T, 8, 128, true>(a, s);
+    else if (a.dh < 128) pa_launch<T, 8, 128, false>(a, s);
+    else if (a.dh == 256) pa_launch<T, 16, 256, true>(a, s);
+    else pa_launch<T, 16, 256, false>(a, s);
 }
 
 extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages,
