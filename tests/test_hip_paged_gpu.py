@@ -372,6 +372,24 @@ def test_attention_gives_a_key_of_score_minus_infinity_no_weight(dtype, dh):
     check_attention(q, k, v, table, lengths - 1, got=got)
 
 
+@pytest.mark.parametrize("dh", list(range(8, 257, 8)))
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_of_every_head_size(dtype, dh):
+    """rows of one wave's tile, of several, and split over workgroups; pages that end inside a tile"""
+    lens = [3, 0, 64, 161, 1200]
+    k, v, table, lengths = make_cache(dtype, 2, dh, 16, lens, seed=dh)
+    check_attention(torch.randn(5, 10, dh, generator=torch.Generator().manual_seed(dh)).to(dtype), k, v, table, lengths)
+
+
+@pytest.mark.parametrize("dh", [72, 88, 120, 136, 192, 256])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_attention_of_wide_heads_by_one_wave_each(dtype, dh):
+    g = torch.Generator().manual_seed(dh)
+    lens = torch.randint(0, 97, (1030,), generator=g).tolist()
+    k, v, table, lengths = make_cache(dtype, 3, dh, 16, lens, seed=dh, M=6)
+    check_attention(torch.randn(1030, 3, dh, generator=g).to(dtype), k, v, table, lengths)
+
+
 def test_attention_reaches_beyond_32_bit_offsets():
     """a pool of 2.2e9 elements (4.5 GB each for K and V): pages at its very end"""
     from vilmedic_amd import ops

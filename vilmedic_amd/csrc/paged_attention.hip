@@ -18,9 +18,13 @@
 //     number, fetched 64 subtiles ahead into a register) plus offsets that no lane ever recomputes.
 //   * two tiles per wave in registers: the next one is requested before the current one is used, and nothing in the walk is loaded behind a condition
 //     (a load in a branch makes the compiler wait for everything in flight).  Worth 6 % at 128 columns.
+//   * heads above 128 columns have no registers for two tiles: K of the next tile is requested once this one's scores are there, V once it is added
+//     up, so one of the two is always in flight (32 rows up to 4000, 4 key heads of 256 columns: 65 us against 72, fp32 121 against 172).
+//   * a head that fills its tile (32, 64, 96, 128, 192, 256 columns) has its size compiled in: every address is one base and constants (fp32 128 columns: 200
+//     registers against 256 and 44 spilled ones; 48 rows up to 8192 289 us against 415).
 //   * long rows are split over workgroups (``splits``); partial (m, l, O) in fp32 go to a workspace and a second launch joins them.  Each row is
 //     split by its OWN length, so the table's width decides only how many workgroups start.
-// Measured: 48 rows of 0 .. 8192 keys, 32 query and 8 key heads of 128 bf16 columns (810 MB of cache): 150 - 153 us with the join, 5.3 TB/s (a large copy: 5.2);
+// Measured: 48 rows of 0 .. 8192 keys, 32 query and 8 key heads of 128 bf16 columns (810 MB of cache): 150 us with the join, 5.4 TB/s (a large copy: 5.2); in fp32 289;
 // one row of 40001 keys, the same heads: 32 us, 5.1 TB/s; 256 rows of up to 128 keys, 12 heads of 64 fp32 columns: 25 us, 4.2 TB/s (short rows: a
 // wave's few tiles do not cover the latency of its first); 64 rows of them in bf16: 7.4 us, three dependent trips to memory and a merge.
 #include "common.h"
@@ -51,13 +55,14 @@ __device__ __forceinline__ float pa_col_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// DK columns of K and Q (a multiple of 32), W columns of V per lane (16 W >= dh; a multiple of W, or of 8 where W is 16, is where a head may end), SUB 16-key subtiles per tile
+// DK columns of K and Q (a multiple of 32), W columns of V per lane (16 W >= dh; one load takes VC of them, side by side over
+// the lanes: a multiple of VC is where a head may end), SUB 16-key subtiles per tile
 template <typename T, int W, int DK> struct PaTile;
 
 template <int W, int DK> struct PaTile<bf16_t, W, DK> {
     static constexpr int SUB = 2, KC = DK / 32;                  // K fragments of 32 columns: 8 per lane
     static constexpr int VD = W / 2;                              // dwords of V per lane and key
-    static constexpr int VC = W < 8 ? W : 8;                      // columns of V per load: a wave's 16 lanes lie side by side in it
+    static constexpr int VC = W < 8 ? W : W == 12 ? 4 : 8;                    // columns of V per load: a wave's 16 lanes lie side by side in it
     struct Q { uint4 q[KC]; };
     uint4 k[SUB][KC];
     uint32_t v[SUB][4][VD];
@@ -94,7 +99,13 @@ template <int W, int DK> struct PaTile<bf16_t, W, DK> {
             if constexpr (VD == 1) v[u][i][0] = *reinterpret_cast<const uint32_t*>(p + min(r * W, dh - W));
             else if constexpr (VD == 3) { const pa_u3 x = *reinterpret_cast<const pa_u3*>(p + min(r * W, dh - W)); v[u][i][0] = x[0]; v[u][i][1] = x[1]; v[u][i][2] = x[2]; }
             else if constexpr (VD == 2) { const uint2 x = *reinterpret_cast<const uint2*>(p + min(r * W, dh - W)); v[u][i][0] = x.x; v[u][i][1] = x.y; }
-            else {
+            else if constexpr (VD == 6) {
+#pragma unroll
+                for (int d = 0; d < VD; d += 2) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p + min(32 * d + r * 4, dh - 4));
+                    v[u][i][d] = x.x; v[u][i][d + 1] = x.y;
+                }
+            } else {
 #pragma unroll
                 for (int d = 0; d < VD; d += 4) {
                     const uint4_t x = pa_ld(p + min(32 * d + r * 8, dh - 8));
@@ -277,29 +288,42 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
     for (int d = 0; d < W; ++d) o[d] = float4_t{0.f, 0.f, 0.f, 0.f};
     const int64_t head = (int64_t)kv << p.shift, page_rows = (int64_t)p.Hk << p.shift;
     const int mask = (1 << p.shift) - 1;
-    auto load = [&](Tile& x, bool (&good)[SUB], int t) {
+    auto place = [&](int64_t (&at)[SUB], bool (&good)[SUB], int t) {
         if (t * SUB >= first + 64) { first = t * SUB; pages = -1; fetch(len); }
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             const int key = t * TK + u * 16, page = __builtin_amdgcn_readlane(pages, (t * SUB - first + u) & 63);
             good[u] = key < len && page >= 0;
-            const int64_t at = ((int64_t)(good[u] ? page : 0) * page_rows + head + (key & mask)) * dh;
-            x.load_k(u, (const T*)p.k + at, r, g, dh);
-            x.load_v(u, (const T*)p.v + at, r, g, dh);
+            at[u] = ((int64_t)(good[u] ? page : 0) * page_rows + head + (key & mask)) * dh;
         }
     };
-    auto use = [&](Tile& x, const bool (&good)[SUB], int t) {
-        bool whole = (t + 1) * TK <= len;
+    auto load_k = [&](Tile& x, const int64_t (&at)[SUB]) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) whole = whole && good[u];
-        float4_t s[SUB];
+        for (int u = 0; u < SUB; ++u) x.load_k(u, (const T*)p.k + at[u], r, g, dh);
+    };
+    auto load_v = [&](Tile& x, const int64_t (&at)[SUB]) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) x.load_v(u, (const T*)p.v + at[u], r, g, dh);
+    };
+    auto load = [&](Tile& x, bool (&good)[SUB], int t) {
+        int64_t at[SUB];
+        place(at, good, t);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) { x.load_k(u, (const T*)p.k + at[u], r, g, dh); x.load_v(u, (const T*)p.v + at[u], r, g, dh); }
+    };
+    auto score = [&](Tile& x, float4_t (&s)[SUB]) {
         if (!WHOLE) x.trim_k(g, dh);
         x.scores(q, s);
-        float mx = m;
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[u][i] *= p.scale_log2;
+    };
+    auto weigh = [&](Tile& x, float4_t (&s)[SUB], const bool (&good)[SUB], int t) {
+        bool whole = (t + 1) * TK <= len;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) whole = whole && good[u];
+        float mx = m;
         if (!whole) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
@@ -329,11 +353,16 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
             for (int i = 0; i < 4; ++i) { s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - base); l += s[u][i]; }
         x.accumulate(s, o);
     };
+    auto use = [&](Tile& x, const bool (&good)[SUB], int t) {
+        float4_t s[SUB];
+        score(x, s);
+        weigh(x, s, good, t);
+    };
     if (t0 < t1) {
         Tile a;
         bool ga[SUB];
         int t = t0;
-        if constexpr (W <= 8) {                                  // the next tile is on its way while this one is worked on
+        if constexpr (W <= 8) {                              // the next tile is on its way while this one is worked on
             Tile b;
             bool gb[SUB];
             load(a, ga, t);
@@ -350,8 +379,21 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
             } else {
                 use(a, ga, t);
             }
-        } else {
-            for (; t < t1; ++t) { load(a, ga, t); use(a, ga, t); }
+        } else {                                                 // K of the next tile while V of this one is worked on, and the other way round
+            load(a, ga, t);
+            for (; t + 1 < t1; ++t) {
+                float4_t s[SUB];
+                int64_t at[SUB];
+                bool gb[SUB];
+                score(a, s);
+                place(at, gb, t + 1);
+                load_k(a, at);
+                weigh(a, s, ga, t);
+                load_v(a, at);
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) ga[u] = gb[u];
+            }
+            use(a, ga, t);
         }
     }
     l = pa_col_sum(l);
@@ -484,6 +526,8 @@ static void pa_launch_w(const PagedAttnArgs& a, hipStream_t s) {
         pa_launch<T, 6, 96, false>(a, s);
     } else if (a.dh == 128) pa_launch<T, 8, 128, true>(a, s);
     else if (a.dh < 128) pa_launch<T, 8, 128, false>(a, s);
+    else if (a.dh == 192) pa_launch<T, 12, 192, true>(a, s);
+    else if (a.dh < 192) pa_launch<T, 12, 192, false>(a, s);
     else if (a.dh == 256) pa_launch<T, 16, 256, true>(a, s);
     else pa_launch<T, 16, 256, false>(a, s);
 }
