@@ -477,14 +477,19 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
 }
 
 // How many workgroups share a row's keys.  The chip's 256 CUs are fed evenly by 256, 512, ... workgroups: one 40001-token row with 8 key heads took 33 us on
-// 160 workgroups, 38 on 320 (64 CUs have twice the work of the others) and 40 on 632.  So: as many rounds of 256 (up to 8) as leave a workgroup
-// 1024 keys of a full row (fewer keys where the rows are short and few: at least 256), shared by the rows; several rows are rarely all full, they get 512 (16
-// rows up to 18000 with 2 key heads 42 -> 38 us, 2 rows up to 20000 with 12 41 -> 36, 48 rows up to 8192 with 8 the same; 256 keys lose again).
-static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
+// 160 workgroups, 38 on 320 (64 CUs have twice the work of the others) and 40 on 632.  So: as many rounds of 256 as leave a workgroup 1024 keys of a
+// full row (fewer keys where the rows are short and few: at least 256), shared by the rows.  Several rows are rarely all full, they get 512 (16 rows up to
+// 18000 with 2 key heads 42 -> 38 us, 2 rows up to 20000 with 12 41 -> 36; 256 keys lose again), and the number of rounds is the nearest one where they are
+// split in any case (4 rows up to 8000 with 8 key heads, 1.95 rounds: 25 -> 22; where a nearest second round would be what brings the join, 360 workgroups
+// of 1024 keys 17 -> 20).  At most 8 rounds (48 rows up to 8192 with 8 key heads 150 us; 5: 158, 16: 154), 12 of heads up to 64 columns, whose keys
+// are half the bytes (64 rows up to 2000 with 12 key heads 49 -> 45, fp32 86 -> 79).
+static int pa_splits(int N, int Hq, int Hkv, int dh, int M, int page_size) {
     const int64_t blocks = (int64_t)N * Hkv * ((Hq / Hkv + 15) / 16);
     const int64_t keys = (int64_t)M * page_size, most = (keys + 255) / 256;
-    int64_t rounds = keys * blocks / (256 * (N > 1 ? 512 : 1024));
-    rounds = rounds < 1 ? 1 : (rounds > 8 ? 8 : rounds);
+    const int64_t round = 256 * (N > 1 ? 512 : 1024);
+    int64_t rounds = (keys * blocks + (blocks <= 128 && N > 1 ? round / 2 : 0)) / round;
+    const int most_rounds = dh <= 64 ? 12 : 8;
+    rounds = rounds < 1 ? 1 : (rounds > most_rounds ? most_rounds : rounds);
     int64_t s = 256 * rounds / blocks;
     if (s > most) s = most;
     if (s > PA_MAX_SPLITS) s = PA_MAX_SPLITS;
@@ -493,7 +498,7 @@ static int pa_splits(int N, int Hq, int Hkv, int M, int page_size) {
 extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, int page_size, int dtype) {
     (void)dtype;
     if (N <= 0 || Hq <= 0 || Hkv <= 0 || M <= 0 || page_size <= 0 || dh <= 0 || Hq % Hkv) return 0;
-    const int s = pa_splits(N, Hq, Hkv, M, page_size);
+    const int s = pa_splits(N, Hq, Hkv, dh, M, page_size);
     return s == 1 ? 0 : (size_t)N * Hq * s * (dh + 2) * sizeof(float);
 }
 
@@ -542,7 +547,7 @@ extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q
                "vm_paged_attention: page_size must be a power of two from 16 on, M * page_size below 2^31 - 2048");
     VM_REQUIRE(dtype == VM_F32 || dtype == VM_BF16, "vm_paged_attention: dtype must be VM_F32 or VM_BF16");
     VM_REQUIRE(((uintptr_t)k_pages % 16) == 0 && ((uintptr_t)v_pages % 16) == 0, "vm_paged_attention: pages must be 16-byte aligned");
-    const int splits = pa_splits(N, Hq, Hkv, M, page_size), qblocks = (Hq / Hkv + 15) / 16;
+    const int splits = pa_splits(N, Hq, Hkv, dh, M, page_size), qblocks = (Hq / Hkv + 15) / 16;
     VM_REQUIRE((int64_t)N * Hq < (1ll << 31) && (int64_t)N * Hkv * qblocks * splits < (1ll << 31), "vm_paged_attention: too many rows x heads");
     const size_t need = vm_paged_attention_ws(N, Hq, Hkv, dh, M, page_size, dtype);
     VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_attention: 16-byte aligned workspace of %zu bytes required", need);
