@@ -241,7 +241,12 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const AttnArgs p, int D
 }
 
 // =============================================================================== dQ  (owner: 16 queries per wave)
-template <int DH, bool RES>
+// delta = sum_j P_j dP_j: where one tile holds every key (ONE), of the very P and dP that dS is made of; elsewhere attn_delta_kernel's rowsum(dO * O), which is the
+// same number with O's rounding to bf16 in it.  That error enters dS_j = P_j (dP_j - delta) with one sign for every key, so it moves dQ along the mean
+// key; where the keys are alike (a deep layer) it is most of dQ's error: 49 keys of 96 columns, last of 12 layers, relative error of the query projection's
+// gradient 0.05 .. 0.11 with it and 0.03 without, and the launch before this one is gone (backward of 256 x 8 heads 82 -> 73 us).  With more tiles a second
+// pass over them would cost the backward 11 .. 30 %.
+template <int DH, bool RES, bool ONE>
 __global__ __launch_bounds__(256, RES ? 4 : ATTN_MIN_BLOCKS) void attn_bwd_dq_kernel(const AttnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int NSLOT = RES ? p.nslot_k : 1;
@@ -258,7 +263,8 @@ __global__ __launch_bounds__(256, RES ? 4 : ATTN_MIN_BLOCKS) void attn_bwd_dq_ke
     float m = 0.f, inv_l = 0.f, delta = 0.f;
     if (qok) {
         const int64_t si = (int64_t)(b * p.H + h) * p.Lq + qrow;
-        m = p.stats[si * 2]; inv_l = 1.0f / p.stats[si * 2 + 1]; delta = p.delta[si];
+        m = p.stats[si * 2]; inv_l = 1.0f / p.stats[si * 2 + 1];
+        if (!ONE) delta = p.delta[si];
     }
     const bf16_t* kbase = p.k + (int64_t)b * p.Lk * p.ldk + h * DH;
     const bf16_t* vbase = p.v + (int64_t)b * p.Lk * p.ldv + h * DH;
@@ -322,8 +328,17 @@ __global__ __launch_bounds__(256, RES ? 4 : ATTN_MIN_BLOCKS) void attn_bwd_dq_ke
                 const float pr = (key < p.Lk && qok) ? __expf(val - m) * inv_l : 0.f;
                 float dpv = dp[f][r];
                 if (p.dropout_p > 0.f) dpv = dropout_keep(drop_key(eff_seed(p.seed, p.seed_dev)), dbase + key, p.thresh) ? dpv * p.drop_scale : 0.f;
-                s[f][r] = pr * (dpv - delta);      // dS^T
+                if constexpr (ONE) { s[f][r] = pr; dp[f][r] = dpv; delta = fmaf(pr, dpv, delta); }
+                else s[f][r] = pr * (dpv - delta);      // dS^T
             }
+        }
+        if constexpr (ONE) {
+            delta = col_sum(delta);
+            if (qok && g == 0) p.delta[(int64_t)(b * p.H + h) * p.Lq + qrow] = delta;      // (for the dK / dV kernel)
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[f][r] *= dp[f][r] - delta;
         }
         bf16x8_t db[2] = {pack_b_operand(s[0], s[1]), pack_b_operand(s[2], s[3])};
 #pragma unroll
@@ -512,13 +527,15 @@ extern "C" int vm_attention_bwd(const void* q, int64_t ldq, const void* k, int64
     // head-resident kernels: delta = rowsum(dO * O) is computed by the dQ kernel (which holds the rows anyway) and saved for dK/dV
     if (dh == 64 && Lk <= 256 && Lq <= 256 && !vm_env().attn_tile && !vm_env().attn_stream) return vm_attn_head_bwd(a, s);
     const int64_t rows = (int64_t)B * H * Lq;
-    hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, dh);
     const dim3 gq((Lq + 63) / 64, H, B), gk((Lk + 63) / 64, H, B);
     const bool resk = Lk <= 256 && !vm_env().attn_stream, resq = Lq <= 256 && !vm_env().attn_stream;
+    const bool one = resk && Lk <= TROWS;
+    if (!one) hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a, dh);
     a.nslot_k = (Lk + 63) / 64; a.nslot_q = (Lq + 63) / 64;
 #define LAUNCH_BWD(D) do { \
-        if (resk) launch_attn(attn_bwd_dq_kernel<D, true>, gq, attn_lds(D, a.nslot_k, 256), s, a); \
-        else launch_attn(attn_bwd_dq_kernel<D, false>, gq, attn_lds(D, 1, 64), s, a); \
+        if (one) launch_attn(attn_bwd_dq_kernel<D, true, true>, gq, attn_lds(D, a.nslot_k, 256), s, a); \
+        else if (resk) launch_attn(attn_bwd_dq_kernel<D, true, false>, gq, attn_lds(D, a.nslot_k, 256), s, a); \
+        else launch_attn(attn_bwd_dq_kernel<D, false, false>, gq, attn_lds(D, 1, 64), s, a); \
         if (resq) launch_attn(attn_bwd_dkv_kernel<D, true>, gk, attn_lds(D, a.nslot_q, 3 * 256 * 4), s, a); \
         else launch_attn(attn_bwd_dkv_kernel<D, false>, gk, attn_lds(D, 1, 3 * 64 * 4), s, a); } while (0)
     switch (dh) { case 32: LAUNCH_BWD(32); break; case 64: LAUNCH_BWD(64); break; case 96: LAUNCH_BWD(96); break; default: LAUNCH_BWD(128); break; }
