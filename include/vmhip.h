@@ -371,6 +371,9 @@ int vm_cast_bf16_to_f32(const void* in, float* out, int64_t n, void* stream);
 int vm_cast_pad_f32_to_bf16(const float* src, void* dst, int rows, int cols, int64_t ld_dst, void* stream);
 int vm_colsum_bf16(const void* x, int64_t ldx, float* out /* += [cols] */, int rows, int cols,
                    const float* scale_dev /* optional device scalar */, void* stream);
+/* the same with the rows split over workgroups; ws: vm_colsum_bf16_ws(rows, cols) bytes, 16-byte aligned (NULL: vm_colsum_bf16) */
+size_t vm_colsum_bf16_ws(int rows, int cols);
+int vm_colsum_bf16_ex(const void* x, int64_t ldx, float* out, int rows, int cols, const float* scale_dev, void* ws, size_t ws_bytes, void* stream);
 int vm_add_bf16(const void* a, const void* b, void* out, int64_t n, void* stream);
 /* out = keep(seed, idx) ? x/(1-p) : 0 with idx = flat element index (the mask vm_gemm_bf16 uses with idx = m*N+n) */
 int vm_dropout_apply_bf16(const void* x, void* out, int64_t n, float p, uint64_t seed, const uint64_t* seed_dev, void* stream);

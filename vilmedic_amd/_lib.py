@@ -109,6 +109,8 @@ SIGNATURES = {
     "vm_cast_bf16_to_f32": (_I, [_P, _P, _L, _P]),
     "vm_cast_pad_f32_to_bf16": (_I, [_P, _P, _I, _I, _L, _P]),
     "vm_colsum_bf16": (_I, [_P, _L, _P, _I, _I, _P, _P]),
+    "vm_colsum_bf16_ws": (_SZ, [_I, _I]),
+    "vm_colsum_bf16_ex": (_I, [_P, _L, _P, _I, _I, _P, _P, _SZ, _P]),
     "vm_add_bf16": (_I, [_P, _P, _P, _L, _P]),
     "vm_dropout_apply_bf16": (_I, [_P, _P, _L, _F, _U64, _P, _P]),
     "vm_feature_mask": (_I, [_P, _P, _I, _I, _P]),

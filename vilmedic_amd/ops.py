@@ -254,8 +254,9 @@ def wgrad(dY, X, dW, *, ld_dy=None, ld_x=None, alpha_dev=None, n_out=None):
 def colsum(x, out, rows=None, cols=None, scale_dev=None):
     rows = rows if rows is not None else x.shape[0]
     cols = cols if cols is not None else x.shape[1]
-    check(lib().vm_colsum_bf16(ptr(x), x.stride(0), ptr(out), rows, cols, ptr(scale_dev) if scale_dev is not None else None,
-                               stream()), "vm_colsum_bf16")
+    ws = torch.empty(lib().vm_colsum_bf16_ws(rows, cols), dtype=torch.uint8, device=x.device)
+    check(lib().vm_colsum_bf16_ex(ptr(x), x.stride(0), ptr(out), rows, cols, ptr(scale_dev) if scale_dev is not None else None, ptr(ws), ws.numel(),
+                                  stream()), "vm_colsum_bf16")
 
 
 # ----------------------------------------------------------------------------- backward marks
