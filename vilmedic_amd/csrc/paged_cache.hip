@@ -62,7 +62,8 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
     __shared__ uint32_t sh[3][WAVES];
     __shared__ int s_taken, s_more;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int head = (p.ring[0] % p.P + p.P) % p.P, count = min(max(p.ring[1], 0), p.P);      // (outside: the caller's error, and no way out of the ring)
+    const int turned = p.ring[0] % p.P, head = turned < 0 ? turned + p.P : turned;            // (no sum above P: two pools of more than 2^30 pages pass 31 bits)
+    const int count = min(max(p.ring[1], 0), p.P);                                            // (outside: the caller's error, and no way out of the ring)
     const int64_t cap = (int64_t)p.M * p.s;
     uint32_t tok_before = 0, want_before = 0, back_before = 0;
     if (tid == 0) s_taken = s_more = 0;
