@@ -31,3 +31,18 @@ def test_plan_on_a_ring_of_more_than_2_30_pages():
         back = torch.tensor([(at + 1000 + k) % P for k in range(3)], device=dev())
         assert free[back].tolist() == pages and ring.tolist() == [(at % P + 3) % P, 1000] and not lengths.any()
         free[back] = back.to(I32)
+
+
+@pytest.mark.parametrize("rows", [2, 1500])
+def test_plan_with_pages_of_more_than_2_30_tokens(rows):
+    """length + page_size passes 2^31 where the page size is no power of two; one launch (2 rows) and two (1500)"""
+    from vilmedic_amd import ops
+    s, length = 1_200_000_000, 1_100_000_000
+    lengths, table = torch.full((rows,), length, dtype=I32, device=dev()), torch.arange(5, 5 + rows, dtype=I32, device=dev())[:, None].contiguous()
+    new = torch.zeros(rows, dtype=I32, device=dev())
+    new[0], new[-1] = 2, 1
+    free, ring = torch.arange(rows + 10, dtype=I32, device=dev()), ints(1, 3)
+    slots, positions, cu, granted = ops.paged_plan(lengths, new, table, free, ring, s, 3)
+    assert positions.tolist() == [length, length + 1, length] and granted.tolist() == new.tolist()
+    assert slots.tolist() == [5 * s + length, 5 * s + length + 1, (4 + rows) * s + length]
+    assert ring.tolist() == [1, 3] and table.flatten().tolist() == list(range(5, 5 + rows)) and lengths.tolist() == (length + new).tolist()

@@ -117,6 +117,8 @@ __device__ __forceinline__ void plan_scan(const PlanArgs& p, PlanRow* rows, int*
         p.ring[1] = count - s_taken + returned;
     }
 }
+// pages of `len` tokens (len, s < 2^31: their sum passes 31 bits where s is no power of two)
+__device__ __forceinline__ int plan_pages(int len, int s) { return (int)(((uint32_t)len + (uint32_t)s - 1) / (uint32_t)s); }
 // head + something below 2 P, taken around the ring (no division: a 64-bit one costs more than everything around it)
 __device__ __forceinline__ int ring_place(int64_t at, int P) { at -= at >= P ? P : 0; return (int)(at - (at >= P ? P : 0)); }
 
@@ -125,7 +127,7 @@ __device__ __forceinline__ int ring_place(int64_t at, int P) { at -= at >= P ? P
 __device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows, const PlanRing g, int tid, int threads) {
     for (int i = tid; i < p.N; i += threads) {
         const PlanRow r = rows[i];
-        if (r.kind == 1 && r.cnt == 1) p.table[(int64_t)i * p.ld_table + (r.len + p.s - 1) / p.s] = p.free_pages[ring_place((int64_t)g.head + r.ofs, p.P)];
+        if (r.kind == 1 && r.cnt == 1) p.table[(int64_t)i * p.ld_table + plan_pages(r.len, p.s)] = p.free_pages[ring_place((int64_t)g.head + r.ofs, p.P)];
     }
     if (!g.more) return;
     int lanes = 64;
@@ -135,7 +137,7 @@ __device__ __forceinline__ void plan_rows(const PlanArgs& p, const PlanRow* rows
         const PlanRow r = rows[i];
         int32_t* row = p.table + (int64_t)i * p.ld_table;
         if (r.kind == 1 && r.cnt > 1) {
-            const int have = (r.len + p.s - 1) / p.s;
+            const int have = plan_pages(r.len, p.s);
             for (int j = lane; j < r.cnt; j += lanes) row[have + j] = p.free_pages[ring_place((int64_t)g.head + r.ofs + j, p.P)];
         } else if (r.kind == 2) {
             for (int j = lane; j < p.M; j += lanes) {
@@ -153,7 +155,7 @@ __device__ __forceinline__ void plan_token(const PlanArgs& p, const PlanRow* row
         while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (cu[mid] <= t) lo = mid; else hi = mid; }
         const PlanRow r = rows[lo];
         if (r.kind == 1) {
-            const int at = r.len + (t - cu[lo]), have = (r.len + p.s - 1) / p.s, col = at / p.s;
+            const int at = r.len + (t - cu[lo]), have = plan_pages(r.len, p.s), col = at / p.s;
             // a page taken in this call is read from the ring: the row of the table may be under construction
             const int page = col >= have ? p.free_pages[ring_place((int64_t)g.head + r.ofs + (col - have), p.P)] : p.table[(int64_t)lo * p.ld_table + col];
             pos = at;
