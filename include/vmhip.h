@@ -442,9 +442,9 @@ int vm_attention_decode_f32(const float* q, int64_t ldq, const float* k, int64_t
  *   - cu_tokens int32 [N + 1]: prefix sums of max(new_tokens, 0), clipped to max_tokens: the packed token order;
  *   - slots int64 [max_tokens]: where token t of the packed order goes, -1 for refused rows and behind the last token; positions int64
  *     [max_tokens]: its position in its request, 0 for those.
- * lengths outside [0, M * page_size] are clamped; page numbers outside [0, P) in the table yield slot -1.  The rows of a table may share no page
- * with each other if they are released through this call.  ws: vm_paged_plan_ws(N, M, max_tokens) bytes, 16-byte
- * aligned, NULL where it is 0.
+ * At most 2^30 rows and tokens; N * M, M * page_size and P stay below 2^31.  lengths outside [0, M * page_size] are clamped; page numbers outside
+ * [0, P) in the table yield slot -1.  The rows of a table may share no page with each other if they are released through this call.  ws:
+ * vm_paged_plan_ws(N, M, max_tokens) bytes, 16-byte aligned, NULL where it is 0.
  * vm_paged_kv_write: k_pages[slot / page_size, h, slot % page_size, :] = k[t, h, :], v likewise; tokens whose slot lies outside
  * [0, P * page_size) are skipped.  k, v: [T, Hkv, dh] with unit column stride, other strides in elements.  The slots of one call must differ.
  * vm_paged_attention: one query token per row, o[n, h] = sum_j softmax_j(scale * q[n, h] . K_j) V_j over j < lengths[n] (clamped to M * page_size)

@@ -195,7 +195,7 @@ extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_
     VM_REQUIRE(lengths && new_tokens && block_table && free_pages && ring && cu_tokens && granted, "vm_paged_plan: null pointer");
     VM_REQUIRE(N > 0 && M > 0 && P > 0 && page_size > 0 && max_tokens >= 0 && ld_table >= M, "vm_paged_plan: bad shape");
     VM_REQUIRE(max_tokens == 0 || (slots && positions), "vm_paged_plan: slots and positions of max_tokens entries required");
-    VM_REQUIRE(max_tokens <= (1 << 30), "vm_paged_plan: max_tokens must be at most 2^30");
+    VM_REQUIRE(max_tokens <= (1 << 30) && N <= (1 << 30), "vm_paged_plan: max_tokens and N must be at most 2^30");       // (the strides of the loops over them stay in 31 bits)
     VM_REQUIRE((int64_t)N * M < (1ll << 31) && (int64_t)M * page_size < (1ll << 31), "vm_paged_plan: N * M and M * page_size must stay below 2^31");
     const size_t need = vm_paged_plan_ws(N, M, max_tokens);
     VM_REQUIRE(need == 0 || (ws && ((uintptr_t)ws % 16) == 0 && ws_bytes >= need), "vm_paged_plan: 16-byte aligned workspace of %zu bytes required", need);
@@ -210,7 +210,7 @@ extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_
         return vm_check_launch("vm_paged_plan");
     }
     hipLaunchKernelGGL(paged_plan_scan_kernel, dim3(1), dim3(PLAN_THREADS), 0, s, a);
-    int blocks = max_tokens > N * 64 ? (max_tokens + 255) / 256 : (N + 3) / 4;
+    int blocks = max_tokens > N * 64ll ? (max_tokens + 255) / 256 : (N + 3) / 4;
     if (blocks > 2048) blocks = 2048;
     if (blocks < 1) blocks = 1;
     hipLaunchKernelGGL(paged_plan_fill_kernel, dim3(blocks), dim3(256), 0, s, a);

@@ -1285,8 +1285,8 @@ def paged_plan(lengths, new_tokens, block_table, free_pages, free_ring, page_siz
         _refuse(name, "at least one row, one column, one page and one token per page")
     if not 0 <= max_tokens <= 1 << 30:
         _refuse(name, f"max_tokens must lie between 0 and 2^30, got {max_tokens}")
-    if N * M >= 1 << 31 or M * page_size >= 1 << 31 or P >= 1 << 31:
-        _refuse(name, "the table's size, M * page_size and the number of pages must stay below 2^31")
+    if N > 1 << 30 or N * M >= 1 << 31 or M * page_size >= 1 << 31 or P >= 1 << 31:
+        _refuse(name, "at most 2^30 rows; the table's size, M * page_size and the number of pages must stay below 2^31")
     other = _elsewhere(lengths)
     if other is not None:
         with other:
