@@ -46,3 +46,48 @@ def test_plan_with_pages_of_more_than_2_30_tokens(rows):
     assert positions.tolist() == [length, length + 1, length] and granted.tolist() == new.tolist()
     assert slots.tolist() == [5 * s + length, 5 * s + length + 1, (4 + rows) * s + length]
     assert ring.tolist() == [1, 3] and table.flatten().tolist() == list(range(5, 5 + rows)) and lengths.tolist() == (length + new).tolist()
+
+
+def test_write_of_more_than_2_24_tokens():
+    from vilmedic_amd import ops
+    T = (1 << 24) + 5
+    k = torch.randint(-100, 100, (T, 1, 8), dtype=torch.int16, device=dev()).view(BF)
+    v = torch.randint(-100, 100, (T, 1, 8), dtype=torch.int16, device=dev()).view(BF)
+    P = -(-T // 16)
+    pages = torch.zeros(2, P, 1, 16, 8, dtype=BF, device=dev())
+    slots = torch.arange(P * 16 - 1, P * 16 - 1 - T, -1, device=dev())
+    ops.paged_kv_write(k, v, pages[0], pages[1], slots)
+    bits = pages.view(torch.int16).view(2, P * 16, 8).flip(1)
+    assert torch.equal(bits[0, :T], k.view(torch.int16)[:, 0]) and torch.equal(bits[1, :T], v.view(torch.int16)[:, 0]) and not bits[:, T:].any()
+
+
+def test_attention_of_more_than_2_26_rows():
+    from vilmedic_amd import ops
+    period, N = 4096, (1 << 26) + 4096
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(period, 1, 8, generator=g).to(BF).to(dev()).repeat(N // period, 1, 1)
+    k, v = (torch.randn(5, 1, 16, 8, generator=g).to(BF).to(dev()) for _ in range(2))
+    table = torch.randint(0, 5, (period, 1), generator=g).to(I32).to(dev()).repeat(N // period, 1)
+    lengths = torch.randint(0, 17, (period,), generator=g).to(I32).to(dev()).repeat(N // period)
+    got = ops.paged_attention(q, k, v, table, lengths)
+    few = ops.paged_attention(q[:period], k, v, table[:period], lengths[:period])         # (a wave per row here too)
+    assert few.abs().sum() > 0
+    assert bool((got.view(N // period, period, 8).view(torch.int16) == few.view(1, period, 8).view(torch.int16)).all())
+
+
+def test_logprobs_of_more_than_2_26_rows():
+    from vilmedic_amd import ops
+    period, R, V = 4096, (1 << 26) + 4096, 16
+    g = torch.Generator().manual_seed(4)
+    x0 = torch.randn(period, V, generator=g).to(BF).to(dev())
+    t0 = torch.randint(-1, V, (period,), generator=g).to(dev())
+    g0 = torch.randn(period, generator=g).to(dev())
+
+    def both(n):
+        x = x0.repeat(n, 1).requires_grad_(True)
+        out = ops.token_logprobs(x, t0.repeat(n), 1)
+        dx, = torch.autograd.grad([out.logp, out.entropy], [x], [g0.repeat(n), torch.ones(n * period, device=dev())])
+        return [out.logp.detach(), out.entropy.detach(), out.top_logp.detach(), out.top_ids, dx]
+    for many, few in zip(both(R // period), both(1)):
+        assert few.abs().sum() > 0
+        assert bool((many.view(R // period, -1) == few.view(1, -1)).all())

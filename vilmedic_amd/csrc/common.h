@@ -12,6 +12,7 @@ typedef __attribute__((ext_vector_type(4))) float float4_t;   // MFMA 16x16 C/D 
 typedef __attribute__((ext_vector_type(4))) uint32_t uint4_t;
 
 #define VM_WAVE 64
+#define VM_MAX_BLOCKS (1ll << 21)     // workgroups per launch: a launch holds fewer than 2^32 threads, of up to 1024 a workgroup; what is longer goes in several
 
 __device__ __forceinline__ float bf16_to_f32(bf16_t h) { return __uint_as_float(((uint32_t)h) << 16); }
 // fp32 -> bf16, round-to-nearest-even (matches torch .to(bfloat16)): the gfx950 hardware convert v_cvt_pk_bf16_f32

@@ -28,6 +28,7 @@
 // one row of 40001 keys, the same heads: 32 us, 5.1 TB/s; 256 rows of up to 128 keys, 12 heads of 64 fp32 columns: 25 us, 4.2 TB/s (short rows: a
 // wave's few tiles do not cover the latency of its first); 64 rows of them in bf16: 7.4 us, three dependent trips to memory and a merge.
 #include "common.h"
+#include <algorithm>
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t pa_u3 __attribute__((ext_vector_type(3), aligned(4)));
@@ -37,6 +38,7 @@ __device__ __forceinline__ uint4_t pa_ld(const void* p) { return __builtin_nonte
 struct PagedAttnArgs {
     const void* q; int64_t q_row, q_head; const void* k; const void* v; const int32_t* table; int64_t ld_table; const int32_t* lengths; void* o;
     float* part_o; float* part_ml; int N, Hq, Hk, G, qblocks, dh, P, shift, M, splits, q_wide; float scale_log2;
+    int first;                 // workgroup number of this launch's first one
 };
 #define PA_WAVES 4             // of a workgroup that shares a row with others
 __device__ __forceinline__ void pa_store(float* p, float v) { *p = v; }
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(64 * WAVES, W <= 8 ? 2 : 1) void paged_attention_ke
     extern __shared__ __attribute__((aligned(16))) float pa_sm[];      // [waves][16][2] (m, l) | [waves][queries][dh] O
     constexpr int SUB = PaTile<T, W, DK>::SUB, TK = 16 * SUB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    int b = blockIdx.x;
+    int b = p.first + blockIdx.x;
     const int split = b % p.splits; b /= p.splits;
     const int qb = b % p.qblocks; b /= p.qblocks;
     const int kv = b % p.Hk, n = b / p.Hk;
@@ -503,11 +505,15 @@ extern "C" size_t vm_paged_attention_ws(int N, int Hq, int Hkv, int dh, int M, i
 }
 
 template <typename T, int W, int DK, bool WHOLE, int WAVES>
-static void pa_launch_waves(const PagedAttnArgs& a, hipStream_t s) {
+static void pa_launch_waves(PagedAttnArgs a, hipStream_t s) {
     const int nq = a.G < 16 ? a.G : 16;
     const size_t lds = sizeof(float) * (WAVES * 32 + (size_t)WAVES * nq * a.dh);
     if (lds > 65536) hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attention_kernel<T, W, DK, WHOLE, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL((paged_attention_kernel<T, W, DK, WHOLE, WAVES>), dim3(a.N * a.Hk * a.qblocks * a.splits), dim3(64 * WAVES), lds, s, a);
+    const int64_t blocks = (int64_t)a.N * a.Hk * a.qblocks * a.splits;
+    for (int64_t first = 0; first < blocks; first += VM_MAX_BLOCKS) {
+        a.first = (int)first;
+        hipLaunchKernelGGL((paged_attention_kernel<T, W, DK, WHOLE, WAVES>), dim3((unsigned)std::min<int64_t>(blocks - first, VM_MAX_BLOCKS)), dim3(64 * WAVES), lds, s, a);
+    }
 }
 // One wave per row and head, without the merge of four, where that alone fills the chip (12 waves for each of its 256 CUs): 256 rows x 12 heads of up to 128
 // fp32 keys 27.8 us against 30.0; 64 rows the other way round, 9.6 us against 7.6.
@@ -554,7 +560,7 @@ extern "C" int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q
     const int e = dtype == VM_F32 ? 4 : 2;
     PagedAttnArgs a = {q, q_row_stride, q_head_stride, k_pages, v_pages, block_table, ld_table, lengths, o, (float*)ws,
                        (float*)ws + (size_t)N * Hq * splits * dh, N, Hq, Hkv, Hq / Hkv, qblocks, dh, P, __builtin_ctz(page_size), M, splits,
-                       (((uintptr_t)q | (uintptr_t)(q_row_stride * e) | (uintptr_t)(q_head_stride * e)) % 16) == 0, scale * 1.4426950408889634f};
+                       (((uintptr_t)q | (uintptr_t)(q_row_stride * e) | (uintptr_t)(q_head_stride * e)) % 16) == 0, scale * 1.4426950408889634f, 0};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_ATTN, 0.0, s, "paged_attn_n%d_h%d_k%d_d%d", N, Hq, Hkv, dh);
     if (dtype == VM_F32) pa_launch_w<float>(a, s);

@@ -5,6 +5,7 @@
 // elements (2 KB for 16 x 64 bf16): the attention kernel reads whole runs, whatever the number of heads.  A token's slot is
 // page * page_size + offset; slots are int64, everything inside a row of the table is int32.
 #include "common.h"
+#include <algorithm>
 
 // ------------------------------------------------------------------ plan
 // Integers only and deterministic.  With s = page_size, L_i = clamp(lengths[i], 0, M s), t_i = max(new_tokens[i], 0):
@@ -224,11 +225,11 @@ extern "C" int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_
 // columns 2.7 us, a launch's latency.
 struct KvWriteArgs {
     const char* k; const char* v; int64_t k_tok, k_head, v_tok, v_head;      // strides in BYTES
-    char* k_pages; char* v_pages; const int64_t* slots; int H, dh, s, esize; int64_t n_slots;
+    char* k_pages; char* v_pages; const int64_t* slots; int H, dh, s, esize; int64_t n_slots, first;
 };
 template <int PIECE>        // bytes a thread moves: 16, or one element
 __global__ __launch_bounds__(256) void paged_kv_write_kernel(const KvWriteArgs p) {
-    const int64_t t = blockIdx.x;
+    const int64_t t = p.first + blockIdx.x;
     const int64_t slot = p.slots[t];
     if (slot < 0 || slot >= p.n_slots) return;
     const int64_t page = slot / p.s;
@@ -254,12 +255,16 @@ extern "C" int vm_paged_kv_write(const void* k, int64_t k_token_stride, int64_t 
     VM_REQUIRE(((uintptr_t)k_pages % 16) == 0 && ((uintptr_t)v_pages % 16) == 0, "vm_paged_kv_write: pages must be 16-byte aligned");
     const int e = dtype == VM_F32 ? 4 : 2;
     KvWriteArgs a = {(const char*)k, (const char*)v, k_token_stride * e, k_head_stride * e, v_token_stride * e, v_head_stride * e, (char*)k_pages, (char*)v_pages,
-                     slots, Hkv, dh, page_size, e, (int64_t)P * page_size};
+                     slots, Hkv, dh, page_size, e, (int64_t)P * page_size, 0};
     const bool wide = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)a.k_tok | (uintptr_t)a.k_head | (uintptr_t)a.v_tok | (uintptr_t)a.v_head) % 16) == 0;
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_DECODE, 4.0 * T * Hkv * (double)dh * e, s, "paged_kv_write_t%d_h%d_d%d", T, Hkv, dh);
-    if (wide) hipLaunchKernelGGL(paged_kv_write_kernel<16>, dim3(T), dim3(256), 0, s, a);
-    else if (e == 4) hipLaunchKernelGGL(paged_kv_write_kernel<4>, dim3(T), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(paged_kv_write_kernel<2>, dim3(T), dim3(256), 0, s, a);
+    for (int64_t first = 0; first < T; first += VM_MAX_BLOCKS) {
+        const dim3 grid((unsigned)std::min<int64_t>(T - first, VM_MAX_BLOCKS));
+        a.first = first;
+        if (wide) hipLaunchKernelGGL(paged_kv_write_kernel<16>, grid, dim3(256), 0, s, a);
+        else if (e == 4) hipLaunchKernelGGL(paged_kv_write_kernel<4>, grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(paged_kv_write_kernel<2>, grid, dim3(256), 0, s, a);
+    }
     return vm_check_launch("vm_paged_kv_write");
 }

@@ -20,6 +20,7 @@
 // whose rows come through one CU each.  The arithmetic (6 operations and an exponential per logit) takes about three quarters of the memory's time.
 #include "common.h"
 #include <float.h>
+#include <algorithm>
 
 // ascending unsigned order of the values; -0 and +0 are one value, every NaN the largest
 __device__ __forceinline__ uint32_t lp_key(float x) {
@@ -90,6 +91,7 @@ __device__ __forceinline__ float lp_sort_wave(float v) {
 struct LogprobArgs {
     const void* x; int64_t ld_outer, ld_inner; int inner;      // row r starts at (r / inner) * ld_outer + (r % inner) * ld_inner
     const int64_t* target; int V, top; float* logp; float* ent; float* stats; float* top_logp; int64_t* top_ids;
+    int first;                                                 // this launch's first row
 };
 
 // running (maximum, sum e, sum e d) of a thread
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
     __shared__ float2 cand[LP_CAND];                            // (value, column as bits)
     __shared__ int s_list[THREADS];
     __shared__ int s_n, s_owners;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = p.first + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
     // whole pieces, and single logits behind them; a row whose pieces would leave too few threads with a maximum for the alternatives' bound is read in
     // single logits altogether (1000000 x 100 bf16, n = 16: 3.0 ms in pieces, all 100 logits candidates, against 0.77)
@@ -302,12 +304,13 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(const LogprobAr
 struct LogprobGradArgs {
     const void* x; int64_t ld_outer, ld_inner; int inner; const int64_t* target; int V, top; const float* stats; const float* ent; const int64_t* top_ids;
     const float* g_logp; const float* g_ent; const float* g_top; void* dx; int64_t ld_dx;
+    int first;
 };
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logprobs_bwd_kernel(const LogprobGradArgs p) {
     using Vec = LpVec<T>;
     constexpr int E = Vec::E;
-    const int r = gridDim.x - 1 - blockIdx.x, tid = threadIdx.x;
+    const int r = p.first + (gridDim.x - 1 - blockIdx.x), tid = threadIdx.x;
     const T* x = (const T*)p.x + (r / p.inner) * p.ld_outer + (r % p.inner) * p.ld_inner;
     T* dx = (T*)p.dx + r * p.ld_dx;
     const int64_t t = p.target[r];
@@ -365,20 +368,22 @@ static int logprob_check(const void* x, int R, int inner, int V, int top, int dt
 // LP_U pieces per thread: 100000 x 1000 bf16 106 us with 64 threads, 144 with 128, 176 with 256, 676 with 1024; 20000 x 8832 bf16 111 with 256, 118 with 512, 184
 // with 1024; 10000 x 8832 fp32 116 / 108 / 120; 8192 x 30522 bf16 169 / 164 / 157.
 #define LP_LAUNCH(KERNEL, THREADS)                                                                                          \
-    do {                                                                                                                    \
-        if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, THREADS>), dim3(R), dim3(THREADS), 0, s, a);                 \
-        else hipLaunchKernelGGL((KERNEL<bf16_t, THREADS>), dim3(R), dim3(THREADS), 0, s, a);                                \
-    } while (0)
+    for (int64_t first = 0; first < R; first += VM_MAX_BLOCKS) {                                                            \
+        const dim3 grid((unsigned)std::min<int64_t>(R - first, VM_MAX_BLOCKS));                                             \
+        a.first = (int)first;                                                                                               \
+        if (dtype == VM_F32) hipLaunchKernelGGL((KERNEL<float, THREADS>), grid, dim3(THREADS), 0, s, a);                    \
+        else hipLaunchKernelGGL((KERNEL<bf16_t, THREADS>), grid, dim3(THREADS), 0, s, a);                                   \
+    }
 
 extern "C" int vm_token_logprobs_fwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
                                      float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids, int dtype, void* stream) {
     if (int rc = logprob_check(logits, R, inner, V, top, dtype, "vm_token_logprobs_fwd")) return rc;
     VM_REQUIRE(targets && logp && entropy && (top == 0 || (top_logp && top_ids)), "vm_token_logprobs_fwd: null pointer");
-    LogprobArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, logp, entropy, stats, top_logp, top_ids};
+    LogprobArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, logp, entropy, stats, top_logp, top_ids, 0};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 4.0 : 2.0) * R * (double)V, s, "token_logprobs_r%d_V%d_k%d", R, V, top);
-    if (V / (dtype == VM_F32 ? 4 : 8) <= 1536 && R >= 2048) LP_LAUNCH(token_logprobs_kernel, 64);
-    else LP_LAUNCH(token_logprobs_kernel, 256);
+    if (V / (dtype == VM_F32 ? 4 : 8) <= 1536 && R >= 2048) { LP_LAUNCH(token_logprobs_kernel, 64) }
+    else { LP_LAUNCH(token_logprobs_kernel, 256) }
     return vm_check_launch("vm_token_logprobs_fwd");
 }
 extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64_t ld_inner, int inner, const int64_t* targets, int R, int V, int top,
@@ -386,13 +391,13 @@ extern "C" int vm_token_logprobs_bwd(const void* logits, int64_t ld_outer, int64
                                      const float* g_top, void* dlogits, int64_t ld_dlogits, int dtype, void* stream) {
     if (int rc = logprob_check(logits, R, inner, V, top, dtype, "vm_token_logprobs_bwd")) return rc;
     VM_REQUIRE(targets && stats && entropy && dlogits && ld_dlogits >= V && (!g_top || top == 0 || top_ids), "vm_token_logprobs_bwd: bad arguments");
-    LogprobGradArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, stats, entropy, top_ids, g_logp, g_entropy, top ? g_top : nullptr, dlogits, ld_dlogits};
+    LogprobGradArgs a = {logits, ld_outer, ld_inner, inner, targets, V, top, stats, entropy, top_ids, g_logp, g_entropy, top ? g_top : nullptr, dlogits, ld_dlogits, 0};
     hipStream_t s = (hipStream_t)stream;
     VmProfScope prof(VM_FAM_LOSS, (dtype == VM_F32 ? 8.0 : 4.0) * R * (double)V, s, "token_logprobs_bwd_r%d_V%d_k%d", R, V, top);
     const int want = V / (dtype == VM_F32 ? 4 : 8) / LP_U;
-    if (want <= 96) LP_LAUNCH(token_logprobs_bwd_kernel, 64);
-    else if (want <= 384) LP_LAUNCH(token_logprobs_bwd_kernel, 256);
-    else if (want <= 704) LP_LAUNCH(token_logprobs_bwd_kernel, 512);
-    else LP_LAUNCH(token_logprobs_bwd_kernel, 1024);
+    if (want <= 96) { LP_LAUNCH(token_logprobs_bwd_kernel, 64) }
+    else if (want <= 384) { LP_LAUNCH(token_logprobs_bwd_kernel, 256) }
+    else if (want <= 704) { LP_LAUNCH(token_logprobs_bwd_kernel, 512) }
+    else { LP_LAUNCH(token_logprobs_bwd_kernel, 1024) }
     return vm_check_launch("vm_token_logprobs_bwd");
 }
