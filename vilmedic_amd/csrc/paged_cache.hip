@@ -251,6 +251,7 @@ extern "C" int vm_paged_kv_write(const void* k, int64_t k_token_stride, int64_t 
                                  void* k_pages, void* v_pages, const int64_t* slots, int T, int Hkv, int dh, int P, int page_size, int dtype, void* stream) {
     VM_REQUIRE(k && v && k_pages && v_pages && slots, "vm_paged_kv_write: null pointer");
     VM_REQUIRE(T > 0 && Hkv > 0 && P > 0 && page_size > 0 && dh > 0 && dh % 8 == 0, "vm_paged_kv_write: bad shape (dh must be a multiple of 8)");
+    VM_REQUIRE((int64_t)Hkv * dh < (1ll << 29), "vm_paged_kv_write: Hkv * dh must stay below 2^29");              // (a token's pieces are counted in 31 bits)
     VM_REQUIRE(dtype == VM_F32 || dtype == VM_BF16, "vm_paged_kv_write: dtype must be VM_F32 or VM_BF16");
     VM_REQUIRE(((uintptr_t)k_pages % 16) == 0 && ((uintptr_t)v_pages % 16) == 0, "vm_paged_kv_write: pages must be 16-byte aligned");
     const int e = dtype == VM_F32 ? 4 : 2;

@@ -1334,8 +1334,8 @@ def paged_kv_write(k, v, k_pages, v_pages, slots):
     if k.dim() != 3 or k.shape != v.shape or k.shape[1] != H or k.shape[2] != dh or v.dtype != k.dtype or v.device != k.device:
         _refuse(name, f"k and v must be [T, {H}, {dh}] like the pages' heads, of one type, got {_desc(k)} and {_desc(v)}")
     T = k.shape[0]
-    if T >= 1 << 31 or P >= 1 << 31:
-        _refuse(name, "fewer than 2^31 tokens and pages are supported")
+    if T >= 1 << 31 or P >= 1 << 31 or H * dh >= 1 << 29:
+        _refuse(name, "fewer than 2^31 tokens and pages, and fewer than 2^29 columns in all heads, are supported")
     ks, vs = k.stride(), v.stride()
     if ks[2] != 1 or vs[2] != 1:
         _refuse(name, f"the columns of k and v must be contiguous, got {_desc(k)} and {_desc(v)}")
