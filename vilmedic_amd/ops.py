@@ -19,6 +19,7 @@ import os
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -1240,6 +1241,14 @@ def _refuse(name, why):
     raise ValueError(f"{name}: {why}")
 
 
+def _refuse_tangents(name, *tensors):
+    """a dual tensor's tangent would be dropped without a word: a derivative of zero"""
+    if getattr(forward_ad, "_current_level", 0) < 0:         # outside every dual_level (unpack_dual finds out too, in 0.3 us a tensor)
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse(name, "it has no forward-mode derivative")
+
+
 def _desc(t):
     return f"{tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}"
 
@@ -1343,6 +1352,7 @@ def paged_kv_write(k, v, k_pages, v_pages, slots):
         _refuse(name, f"slots must be a contiguous int64 tensor of the {T} tokens on their device, got {_desc(slots)}")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         _refuse(name, "it has no backward pass: call it under torch.no_grad()")
+    _refuse_tangents(name, k, v, k_pages, v_pages)
     if T == 0:
         return
     other = _elsewhere(k)
@@ -1378,6 +1388,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
         _refuse(name, "M * page_size must stay below 2^31 - 2048, N * Hq and the number of pages below 2^31")
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         _refuse(name, "it has no backward pass: call it under torch.no_grad()")
+    _refuse_tangents(name, q, k_pages, v_pages)
     if N == 0:
         return torch.empty_like(q)
     other = _elsewhere(q)
@@ -1455,6 +1466,7 @@ def token_logprobs(logits, targets, top=0):
         _refuse(name, f"top must lie between 0 and min(V, {MAX_TOP_LOGPROBS}), got {top} (V = {V})")
     if V >= 1 << 30 or targets.numel() >= 1 << 31:
         _refuse(name, "fewer than 2^30 columns and 2^31 rows are supported")
+    _refuse_tangents(name, logits)
     if targets.numel() == 0:
         z = logits.float().sum(-1)
         return TokenLogprobs(z, z.clone(), z.new_zeros(*shape, top), targets.new_zeros(*shape, top))
