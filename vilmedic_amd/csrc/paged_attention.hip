@@ -139,16 +139,17 @@ template <int W, int DK> struct PaTile<bf16_t, W, DK> {
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[u][c]), __builtin_bit_cast(bf16x8_t, x.q[c]), s[u], 0, 0, 0);
         }
     }
-    // O^T += V^T P^T.  A probability goes in as two bf16 parts, hi (truncated) + lo: one bf16 would cost 2^-9 of every probability; the second
-    // product is free next to the loads.  hi is taken from p (1 - 2^-9), so that lo is positive wherever p is: an infinite V then stays infinite
-    // (0 * inf would make it NaN); what is left out is below 2^-16 of p.
+    // O^T += V^T P^T.  A probability goes in as two bf16 parts, hi (truncated) + lo: one bf16 would cost 2^-8 of every probability; the second
+    // product is free next to the loads.  hi is the truncation of p less 128 steps of fp32 (2^-16 .. 2^-17 of p), so that lo is positive wherever p is: an
+    // infinite V then stays infinite (0 * inf would make it NaN).  With p in [1, 2) lo lies below 2^-7 + 2^-16; under 2^-7 its own rounding is at
+    // most 2^-16, above it goes to 2^-7: what is left out is at most 2^-16 of p.
     __device__ __forceinline__ void accumulate(const float4_t (&p)[SUB], float4_t (&o)[W]) const {
         uint4 hi, lo;
         uint32_t h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float a = p[e >> 1][2 * (e & 1)], b = p[e >> 1][2 * (e & 1) + 1];
-            const uint32_t ah = __float_as_uint(a * (1.f - 1.f / 512)) & 0xffff0000u, bh = __float_as_uint(b * (1.f - 1.f / 512)) & 0xffff0000u;
+            const uint32_t ah = __builtin_elementwise_sub_sat(__float_as_uint(a), 0x80u) & 0xffff0000u, bh = __builtin_elementwise_sub_sat(__float_as_uint(b), 0x80u) & 0xffff0000u;
             h[e] = (ah >> 16) | bh;
             l[e] = pack_bf16x2(a - __uint_as_float(ah), b - __uint_as_float(bh));
         }
