@@ -103,8 +103,7 @@ class _CausalLM(nn.Module):
                                                       banned=banned, top_k=top_k)
             return ModelOutput(loss=loss, logits=logits, past_key_values=None, hidden_states=None, attentions=None,
                                cross_attentions=None, row_logp=row_logp)
-        B, L, D = h.shape
-        logits = ops.lm_logits_f32(h.reshape(B * L, D), emb_sh, bias, V).view(B, L, V)
+        logits = ops.lm_logits(h, emb_sh, bias, V, g_emb=_rows(arena.grad(emb), V), g_bias=arena.grad(bias))
         return ModelOutput(loss=None, logits=logits, past_key_values=None, hidden_states=None, attentions=None, cross_attentions=None)
 
 

@@ -111,8 +111,7 @@ class BertGenerationDecoder(nn.Module):
             return ModelOutput(loss=loss, logits=logits, past_key_values=None, hidden_states=None, attentions=None,
                                cross_attentions=None, row_logp=row_logp)
         else:
-            B, L, D = h.shape
-            logits = ops.lm_logits_f32(h.reshape(B * L, D), emb_sh, self.lm_head.bias, V).view(B, L, V)
+            logits = ops.lm_logits(h, emb_sh, self.lm_head.bias, V, g_emb=_rows(arena.grad(emb), V), g_bias=arena.grad(self.lm_head.bias))
         return ModelOutput(loss=loss, logits=logits, past_key_values=None, hidden_states=None, attentions=None,
                            cross_attentions=None)
 

@@ -1216,6 +1216,48 @@ def lm_logits_f32(h2, emb_sh, bias, V):
     return out[:, :V]
 
 
+class LmLogitsFn(Fn):
+    """fp32 logits = h E^T + b that carry a gradient: what a loss of the caller's own (token_logprobs' log probabilities and entropies, say) needs from a
+    decoder.  The incoming gradient is rounded to bf16 once, into rows padded with zeros, and runs through the LM head's dgrad / wgrad GEMMs."""
+
+    @staticmethod
+    def forward(ctx, h, emb_sh, bias, V, g_emb, g_bias):
+        B, L, D = h.shape
+        h2 = _2d(h)
+        out = lm_logits_f32(h2, emb_sh, bias, V)
+        ctx.save_for_backward(h2, emb_sh)
+        ctx.meta = (B, L, D, V, g_emb, g_bias)
+        # (its own tensor and no view of the padded one: a view made in here could not be changed in place, logits[..., 0] = -inf)
+        ld = out.stride(0)
+        return torch.empty(0, dtype=out.dtype, device=out.device).set_(out.untyped_storage(), 0, (B, L, V), (L * ld, ld, 1))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        h2, emb_sh = ctx.saved_tensors
+        B, L, D, V, g_emb, g_bias = ctx.meta
+        M, Vp = B * L, emb_sh.shape[0]
+        dlogits = torch.empty(M, Vp, dtype=BF16, device=h2.device)
+        dlogits[:, :V].copy_(g.reshape(M, V))
+        if Vp != V:
+            dlogits[:, V:].zero_()             # (dh contracts over all Vp columns)
+        if g_emb is not None:
+            param_grads(dlogits, h2, g_emb, g_bias, cols=V)
+        dh = None
+        if ctx.needs_input_grad[0]:
+            dh = torch.empty(M, D, dtype=BF16, device=h2.device)
+            gemm(dlogits, 0, emb_sh, 1, dh, M, D, Vp)
+            dh = dh.view(B, L, D)
+        return (dh,) + (None,) * 5
+
+
+def lm_logits(h, emb_sh, bias, V, g_emb=None, g_bias=None):
+    """fp32 logits [B, L, V] of a whole sequence, differentiable where grad mode asks for it"""
+    if torch.is_grad_enabled() and h.requires_grad:
+        return LmLogitsFn.apply(h, emb_sh, bias, V, g_emb, g_bias)
+    return lm_logits_f32(_2d(h), emb_sh, bias, V).view(*h.shape[:-1], V)
+
+
 # ----------------------------------------------------------------------------- paged key-value cache (serving)
 # One decode step of a ragged batch:  paged_plan (pages, slots, positions of the new tokens) -> paged_kv_write -> paged_attention, the last two once
 # per layer.  The cache of a layer is k_pages, v_pages [P, Hkv, page_size, dh]; block_table int32 [N, M] and lengths int32 [N] are shared by
