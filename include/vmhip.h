@@ -467,7 +467,8 @@ int vm_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
  *   logp[r] = x_t - z (0 for a target < 0, NaN for a target >= V), entropy[r] = -sum_c p_c log p_c,
  *   stats [R, 2] = (max x, z - max x): what the backward pass needs of the row (may be NULL without one),
  *   top_ids / top_logp [R, top]: the ``top`` (<= VM_MAX_TOP_LOGPROBS) largest logits of the row, largest first, equal ones by ascending column.
- * Logits of -inf are columns that do not exist (p = 0); a row of nothing else gives -inf, entropy 0, gradient 0.  The per-token scores of
+ * Logits of -inf are columns of p = 0: their gradient is that of a logp / top_logp of their own, if any (as log_softmax has it); a row of nothing
+ * else gives -inf, entropy 0, gradient 0.  The per-token scores of
  * hf:generation/utils.py compute_transition_scores and the policy term of ref:vilmedic/blocks/rl/SCST.py:14-45.
  * vm_token_logprobs_bwd: dlogits (rows ld_dlogits apart, the logits' type) = d/dx sum_r (g_logp logp + g_entropy entropy + sum_k g_top top_logp);
  * each of the three gradients may be NULL (= 0). */

@@ -2,8 +2,8 @@
 // three with respect to the logits.  Per row x of V logits, target t:
 //   z = log sum exp(x)      logp = x_t - z      H = log s - (sum_c e_c d_c) / s   with d_c = x_c - m, e_c = exp(d_c), s = sum e_c, m = max x
 //   top: the n largest logits, largest first, equal ones by ascending column (a NaN counts as the largest, as torch.topk has it), as x_c - z
-// A target < 0 is no token (logp 0, no gradient from it); a target >= V makes its logp NaN.  A row without a logit above -inf has
-// logp -inf, entropy 0, alternatives -inf, gradient 0.
+// A target < 0 is no token (logp 0, no gradient from it); a target >= V makes its logp NaN.  A column at -inf has p = 0: its gradient is that of a logp or an
+// alternative of its own, if any (as log_softmax has it).  A row without a logit above -inf has logp -inf, entropy 0, alternatives -inf, gradient 0.
 //
 // Forward: ONE pass over the row with a running maximum per thread (sums rescaled when it grows: sum e d becomes f (sum e d + delta sum e) with
 // delta = m_old - m_new, f = exp(delta)), 4 x 16 B per thread in flight; m and log s leave the kernel apart, because m + log s in one float loses

@@ -1496,7 +1496,9 @@ def token_logprobs(logits, targets, top=0):
     """Log probability of ``targets`` int64 [...] under softmax(``logits`` [..., V], float32 or bfloat16), the entropy of each distribution and its ``top``
     (<= 32) most likely columns (largest first, equal logits by ascending column), differentiable with respect to the logits through all three.
     A negative target is no token (logp 0, no gradient from it), one from V on gives NaN.  Columns at -inf (banned tokens, a top-k filter) have
-    probability 0 and gradient 0; a row of nothing else gives log probabilities -inf, entropy 0 and gradient 0.  Statistics are fp32 throughout.
+    probability 0 and no gradient but from a log probability of their own: a banned target, or an alternative where fewer columns are left, passes its incoming
+    gradient on as log_softmax does.  A row of nothing else gives log probabilities -inf, entropy 0 and gradient 0.  Statistics are fp32 throughout.
+    No second and no forward-mode derivatives.
     -> TokenLogprobs(logp, entropy, top_logp, top_ids)"""
     name = "token_logprobs"
     if logits.dtype not in _DT:
