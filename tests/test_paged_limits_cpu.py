@@ -51,3 +51,16 @@ def test_forward_mode_derivatives_are_refused_and_not_dropped(which):
             for name in meant:
                 with torch.set_grad_enabled(grad), pytest.raises(ValueError, match=name + ".*forward-mode"):
                     calls[name]()
+
+
+@pytest.mark.parametrize("kw", [dict(kv_page_size=0), dict(kv_page_size=24), dict(kv_page_size=8), dict(kv_page_size=-16), dict(kv_pages=0), dict(kv_pages=-3)])
+def test_generate_refuses_page_sizes_and_pools(kw):
+    from vilmedic_amd.generation import generate
+
+    class Cfg:
+        eos_token_id, pad_token_id, bos_token_id = 2, 1, 0
+
+    class Dec:
+        config = Cfg()
+    with pytest.raises(ValueError, match="kv_page_size must be"):
+        generate(Dec(), input_ids=torch.zeros(2, 1, dtype=torch.long), encoder_hidden_states=torch.zeros(2, 3, 8), kv_cache="paged", **kw)

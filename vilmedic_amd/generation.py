@@ -724,7 +724,10 @@ def generate(decoder, input_ids=None, encoder_hidden_states=None, encoder_attent
     if args.get("kv_cache") not in (None, "contiguous"):
         if args["kv_cache"] != "paged":
             raise ValueError(f"kv_cache must be 'contiguous' or 'paged', got {args['kv_cache']!r}")
-        paged = (int(args.get("kv_page_size") or 16), None if args.get("kv_pages") is None else int(args["kv_pages"]))
+        page = 16 if args.get("kv_page_size") is None else int(args["kv_page_size"])
+        paged = (page, None if args.get("kv_pages") is None else int(args["kv_pages"]))
+        if page < 16 or page & (page - 1) or (paged[1] is not None and paged[1] < 1):
+            raise ValueError(f"kv_page_size must be a power of two from 16 on and kv_pages at least 1, got {page} and {paged[1]}")
     if args.get("output_logprobs") is not None and not ret_dict:
         raise ValueError("output_logprobs needs return_dict_in_generate=True")
     if input_ids is None:
