@@ -564,8 +564,11 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
             if output_logprobs is not None:
                 logprobs.append(ops.token_logprobs(logits, nxt, output_logprobs))
             cur += 1
-            if cur % 8 == 0 and not bool(unf.any()):           # host sync only every 8 steps; trimmed exactly below
-                break
+            if cur % 8 == 0:                                   # host sync only every 8 steps; trimmed exactly below
+                if paged is not None:
+                    st.check_pages()                           # (a pool that is too small ends the call here, not behind its last step)
+                if not bool(unf.any()):
+                    break
     # The one selection kernel covers every call the reference's shipped configs make (greedy; multinomial sampling with bad_words [[pad],[bos]]
     # and an optional top_k <= 256: ref:blocks/rl/SCST.py:142-157).  Outside its domain -- ``output_scores``, top_k > 256 (the YAML value is
     # free), more than 4 bad words, a greedy call with bad words -- the loop below serves the same contract step by step: HF's logits
@@ -599,8 +602,11 @@ def sample(decoder, input_ids, enc, enc_mask, *, max_length, eos_token_id, pad_t
         seq[:, cur] = nxt
         unfinished = unfinished & (nxt != eos_token_id)
         cur += 1
-        if cur % 8 == 0 and not bool(unfinished.any()):      # host sync only every 8 steps; trimmed exactly below
-            break
+        if cur % 8 == 0:                                     # host sync only every 8 steps; trimmed exactly below
+            if paged is not None:
+                st.check_pages()
+            if not bool(unfinished.any()):
+                break
     if paged is not None:
         st.check_pages()
     # exact HF stopping point: generation ends right after the step at which the last row finished
