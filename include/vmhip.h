@@ -448,8 +448,9 @@ int vm_attention_decode_f32(const float* q, int64_t ldq, const float* k, int64_t
  * vm_paged_kv_write: k_pages[slot / page_size, h, slot % page_size, :] = k[t, h, :], v likewise; tokens whose slot lies outside
  * [0, P * page_size) are skipped.  k, v: [T, Hkv, dh] with unit column stride, other strides in elements.  The slots of one call must differ.
  * vm_paged_attention: one query token per row, o[n, h] = sum_j softmax_j(scale * q[n, h] . K_j) V_j over j < lengths[n] (clamped to M * page_size)
- * of key head h / (Hq / Hkv); keys of pages outside [0, P) do not exist; no key at all: zeros.  dh a multiple of 8 up to 256, page_size a power of
- * two from 16 on.  q: unit column stride; o: contiguous [N, Hq, dh].  ws: vm_paged_attention_ws(...) bytes, 16-byte aligned, NULL where it is 0. */
+ * of key head h / (Hq / Hkv); keys of pages outside [0, P) do not exist; no key at all, or none with a score above -inf: zeros.  dh a multiple of 8
+ * up to 256, page_size a power of two from 16 on.  q: unit column stride; o: contiguous [N, Hq, dh].  ws: vm_paged_attention_ws(...) bytes, 16-byte
+ * aligned, NULL where it is 0. */
 size_t vm_paged_plan_ws(int N, int M, int max_tokens);
 int vm_paged_plan(int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int64_t ld_table, int N, int M, int32_t* free_pages, int32_t* ring,
                   int P, int page_size, int64_t* slots, int64_t* positions, int max_tokens, int32_t* cu_tokens, int32_t* granted, void* ws,

@@ -91,3 +91,21 @@ def test_logprobs_of_more_than_2_26_rows():
     for many, few in zip(both(R // period), both(1)):
         assert few.abs().sum() > 0
         assert bool((many.view(R // period, -1) == few.view(1, -1)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dh,length", [(64, 1), (64, 40), (40, 33), (64, 9000), (192, 70)])
+def test_attention_of_rows_whose_scores_are_all_minus_infinity(dtype, dh, length):
+    """no key with a score above -inf: zeros, also where the values are infinite (and in one launch as well as in split rows)"""
+    from vilmedic_amd import ops
+    M = -(-length // 16)
+    k, v = torch.zeros(M + 1, 2, 16, dh, dtype=dtype, device=dev()), torch.ones(M + 1, 2, 16, dh, dtype=dtype, device=dev())
+    k[..., dh - 1] = -float("inf")
+    v[:, 1] = float("inf")
+    q = torch.ones(2, 4, dh, dtype=dtype, device=dev())
+    table = torch.arange(1, M + 1, dtype=I32, device=dev()).expand(2, M).contiguous()
+    lengths = ints(length, length)
+    assert not ops.paged_attention(q, k, v, table, lengths).any()
+    k[1, :, 0] = 0                                            # one key of weight 1 in page 1, which both rows start with
+    out = ops.paged_attention(q, k, v, table, lengths)
+    assert bool((out[:, :2] == 1).all())

@@ -1408,8 +1408,8 @@ def paged_kv_write(k, v, k_pages, v_pages, slots):
 def paged_attention(q, k_pages, v_pages, block_table, lengths, scale=None):
     """Attention of one new token per row over its paged history: ``q`` [N, Hq, dh] (unit column stride; Hq a multiple of the pages' Hkv heads: query head h
     reads key head h // (Hq / Hkv)), pages [P, Hkv, page_size, dh], ``block_table`` int32 [N, M], ``lengths`` int32 [N] (the new token's own key included,
-    if it is to see itself).  ``scale`` defaults to dh ** -0.5.  -> [N, Hq, dh] in q's type; a row of length 0 gives zeros, keys in pages that
-    do not exist (numbers outside [0, P)) are left out, stale values behind a row's length are never read into a result."""
+    if it is to see itself).  ``scale`` defaults to dh ** -0.5.  -> [N, Hq, dh] in q's type; a row of length 0, or without a score above
+    -inf, gives zeros, keys in pages that do not exist (numbers outside [0, P)) are left out, stale values behind a row's length do not reach a result."""
     name = "paged_attention"
     P, H, s, dh, dt = _check_pages(name, k_pages, v_pages, q)
     if q.dim() != 3 or q.shape[2] != dh or q.shape[1] < 1 or q.shape[1] % H:
